@@ -1,0 +1,54 @@
+// Operators of a decode step: the paged key-value cache (paged_append.cu, paged_attention.cu) and linear layers with 4-bit
+// weights (matmul_w4.cu).  Arguments as in include/gc_b200.h; the launchers check them and throw.
+#pragma once
+#include <cstddef>
+#include <cstdint>
+#include <cuda_runtime.h>
+
+#include "../../include/gc_b200.h"
+#include "paged_index.h"
+
+namespace gcb {
+
+// What the kernels of the cache see.  Strides in bytes.
+struct PagedCache {
+  uint8_t *keys, *values;
+  int64_t key_page, key_head, key_token, value_page, value_head, value_token;
+  const float *key_scale, *value_scale;
+  PageTable table;
+  int kv_heads, dim;
+  int *error;
+};
+// Checks a descriptor; `writes`: the call stores into the cache.
+PagedCache checked_cache(const gcb200_paged_cache &c, bool writes);
+
+struct AppendArgs {
+  const void *q, *k, *v;
+  void *q_out;
+  int64_t q_stride[2], k_stride[2], v_stride[2], q_out_stride[2], heads, tokens, rotary_dim;
+  const int32_t *sequences, *positions;
+  const double *inv_freq;
+  int interleaved;
+};
+void paged_kv_append(const gcb200_paged_cache &cache, const AppendArgs &a, cudaStream_t stream);
+
+struct PagedAttentionArgs {
+  const void *q;
+  void *out;
+  int64_t q_stride[2], out_stride[2], heads, window;
+  const int32_t *lengths;
+  float scale;
+  float *lse;
+  void *workspace;
+  size_t workspace_bytes;
+};
+size_t paged_attention_workspace(int64_t heads, int64_t kv_heads, int64_t head_dim);
+void paged_attention(const gcb200_paged_cache &cache, const PagedAttentionArgs &a, cudaStream_t stream);
+
+size_t w4_packed_bytes(int64_t N, int64_t K, int64_t group, int has_zeros);
+void w4_pack(const uint8_t *codes, int64_t codes_stride, const void *scales, int64_t scales_stride, const uint8_t *zeros,
+             int64_t zeros_stride, int64_t N, int64_t K, int64_t group, void *packed, cudaStream_t stream);
+void matmul_w4(int dtype, const void *X, int64_t ldx, const void *packed, const void *bias, void *Y, int64_t ldy, int64_t M,
+               int64_t N, int64_t K, int64_t group, int has_zeros, int relu, cudaStream_t stream);
+
+} // namespace gcb

@@ -1,0 +1,316 @@
+// Appending to a paged key-value cache: k (rotated) and v of new tokens into their pages, q rotated beside them.
+//
+// A rotation turns pair (a, b) of a query or key by angle = position * inv_freq[i]:
+//   (a, b) -> (a cos - b sin, b cos + a sin)
+// The angle of a far position has no bits of its fraction left in f32 (position 10^6: the spacing is 0.06), so it is formed in
+// f64 in whole turns, reduced by the whole turns there, and only the remaining fraction becomes f32 for sincospi.  All heads of
+// a token share its angles: a block computes them once, into shared memory.
+//
+// Bound by HBM: q read and written, k and v read, the cache's rows written.
+#include "decode_ops.h"
+
+#include <algorithm>
+#include <stdexcept>
+#include <string>
+
+#include "mma_ptx.cuh"
+#include "runtime.h"
+
+namespace gcb {
+
+namespace {
+
+constexpr int kAppendThreads = 256;
+constexpr int kMaxDim = 256;
+
+struct AppendParams {
+  PagedCache c;
+  const uint16_t *q, *k, *v;
+  uint16_t *q_out;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;   // elements
+  const int32_t *sequences, *positions;
+  const double *inv_freq;
+  int heads, rotary, interleaved, units;   // units: pieces of a row, two chunks each
+};
+
+// VEC consecutive 16-bit elements as they lie in memory; ALIGNED: moved in one access.  VEC 1 fills the low half of a word.
+template <int VEC> struct Chunk {
+  uint32_t w[(VEC + 1) / 2];
+};
+template <int VEC, bool ALIGNED> __device__ __forceinline__ Chunk<VEC> load(const uint16_t *p) {
+  Chunk<VEC> x;
+  if constexpr (ALIGNED && VEC == 8) {
+    const uint4 u = *reinterpret_cast<const uint4 *>(p);
+    x.w[0] = u.x; x.w[1] = u.y; x.w[2] = u.z; x.w[3] = u.w;
+  } else if constexpr (ALIGNED && VEC == 4) {
+    const uint2 u = *reinterpret_cast<const uint2 *>(p);
+    x.w[0] = u.x; x.w[1] = u.y;
+  } else if constexpr (VEC == 1) {
+    x.w[0] = p[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) x.w[i] = p[2 * i] | (uint32_t(p[2 * i + 1]) << 16);
+  }
+  return x;
+}
+template <int VEC, bool ALIGNED> __device__ __forceinline__ void store(uint16_t *p, const Chunk<VEC> &x) {
+  if constexpr (ALIGNED && VEC == 8) *reinterpret_cast<uint4 *>(p) = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
+  else if constexpr (ALIGNED && VEC == 4) *reinterpret_cast<uint2 *>(p) = make_uint2(x.w[0], x.w[1]);
+  else if constexpr (VEC == 1) p[0] = uint16_t(x.w[0]);
+  else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {
+      p[2 * i] = uint16_t(x.w[i]);
+      p[2 * i + 1] = uint16_t(x.w[i] >> 16);
+    }
+  }
+}
+template <bool BF16, int VEC> __device__ __forceinline__ void unpack(const Chunk<VEC> &c, float (&x)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) x[i] = half_to_f32<BF16>((c.w[i / 2] >> (16 * (i & 1))) & 0xFFFFu);
+}
+template <bool BF16, int VEC> __device__ __forceinline__ Chunk<VEC> pack(const float (&x)[VEC]) {
+  Chunk<VEC> c;
+#pragma unroll
+  for (int i = 0; i < (VEC + 1) / 2; ++i) c.w[i] = pack_half2<BF16>(x[2 * i], VEC > 1 ? x[VEC > 1 ? 2 * i + 1 : 0] : 0.f);
+  return c;
+}
+// 8-bit codes of x / scale.  The quotient is a true division: a product with the reciprocal would round twice.
+template <int VEC, bool ALIGNED> __device__ __forceinline__ void store_e4m3(uint8_t *p, const float (&x)[VEC], float scale) {
+  if constexpr (ALIGNED) {
+    uint32_t w[VEC / 4];
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i)
+      w[i] = f32x2_to_e4m3x2(__fdiv_rn(x[4 * i], scale), __fdiv_rn(x[4 * i + 1], scale)) |
+             (f32x2_to_e4m3x2(__fdiv_rn(x[4 * i + 2], scale), __fdiv_rn(x[4 * i + 3], scale)) << 16);
+    if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t *>(p) = w[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) p[i] = uint8_t(f32x2_to_e4m3x2(__fdiv_rn(x[i], scale), 0.f));
+  }
+}
+
+// A thread's piece of a row: two chunks of VEC elements, the partners of a rotation by halves or neighbours.
+struct Piece {
+  const uint16_t *src;
+  uint16_t *dst;
+  float scale;
+  int d0, d1;          // first elements of the chunks; d1 may lie behind the row
+  bool live, cached, rotated, partners;
+};
+template <bool F8, int VEC> __device__ __forceinline__ Piece piece_of(const AppendParams &p, int u, int64_t t, int page, int slot) {
+  const PagedCache &c = p.c;
+  Piece x;
+  const int q_rows = p.q ? p.heads : 0, row = u / p.units, half = p.rotary >> 1;
+  int i = u - row * p.units;
+  x.live = row < q_rows + 2 * c.kv_heads;
+  x.cached = row >= q_rows;
+  x.rotated = p.rotary > 0;
+  x.scale = 1.f;
+  x.src = nullptr;
+  x.dst = nullptr;
+  if (!x.cached) {
+    x.src = p.q + t * p.q_token + row * p.q_head;
+    x.dst = p.q_out + t * p.o_token + row * p.o_head;
+  } else if (x.live && page >= 0) {
+    const int r = row - q_rows, head = r < c.kv_heads ? r : r - c.kv_heads;
+    if (r < c.kv_heads) {
+      x.src = p.k + t * p.k_token + head * p.k_head;
+      x.dst = reinterpret_cast<uint16_t *>(c.keys + page * c.key_page + head * c.key_head + slot * c.key_token);
+      if (F8 && c.key_scale) x.scale = c.key_scale[head];
+    } else {
+      x.src = p.v + t * p.v_token + head * p.v_head;
+      x.dst = reinterpret_cast<uint16_t *>(c.values + page * c.value_page + head * c.value_head + slot * c.value_token);
+      if (F8 && c.value_scale) x.scale = c.value_scale[head];
+      x.rotated = false;
+    }
+  } else {
+    x.live = false;
+  }
+  const bool halves = x.rotated && !p.interleaved;
+  x.partners = halves && i * VEC < half;
+  if (x.partners) {
+    x.d0 = i * VEC;
+    x.d1 = x.d0 + half;
+  } else {
+    if (halves) i -= half / VEC;
+    x.d0 = (halves ? p.rotary : 0) + 2 * i * VEC;
+    x.d1 = x.d0 + VEC;
+  }
+  if (x.d0 >= c.dim) x.live = false;
+  return x;
+}
+
+// One block per token.
+template <bool BF16, bool F8, int VEC, bool ALIGNED>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendParams p) {
+  __shared__ float2 turn[kMaxDim / 2];   // (cos, sin) of each pair
+  pdl_wait();
+  pdl_launch_dependents();
+  const PagedCache &c = p.c;
+  const int t = blockIdx.x;
+  const int seq = p.sequences ? p.sequences[t] : t, pos = p.positions[t];
+  if (seq < 0 || pos < 0) return;   // padding
+  const int half = p.rotary >> 1;
+  for (int i = threadIdx.x; i < half; i += kAppendThreads) {
+    const double turns = double(pos) * p.inv_freq[i] * 0.15915494309189533577;   // 1 / (2 pi)
+    float s, co;
+    sincospif(2.f * float(turns - rint(turns)), &s, &co);
+    turn[i] = make_float2(co, s);
+  }
+  const int slot = pos % c.table.page_size, page = page_of(c.table, seq, pos);
+  if (page < 0 && threadIdx.x == 0) atomicExch(c.error, int(ERR_BAD_PAGE));
+  __syncthreads();
+
+  const int rows = (p.q ? p.heads : 0) + 2 * c.kv_heads;
+  for (int u = threadIdx.x; u < rows * p.units; u += kAppendThreads) {
+    const Piece x = piece_of<F8, VEC>(p, u, t, page, slot);
+    if (!x.live) continue;
+    const bool both = x.d1 < c.dim;
+    Chunk<VEC> ca = load<VEC, ALIGNED>(x.src + x.d0), cb = ca;
+    if (both) cb = load<VEC, ALIGNED>(x.src + x.d1);
+    if (x.rotated || (F8 && x.cached)) {
+      float a[VEC], b[VEC];
+      unpack<BF16, VEC>(ca, a);
+      unpack<BF16, VEC>(cb, b);
+      if (x.partners) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float2 w = turn[x.d0 + i];
+          const float f = a[i], g = b[i];
+          a[i] = f * w.x - g * w.y;
+          b[i] = g * w.x + f * w.y;
+        }
+      } else if (x.rotated && p.interleaved) {
+        if constexpr (VEC >= 2) {
+#pragma unroll
+          for (int i = 0; i < VEC; i += 2) {
+            if (x.d0 + i < p.rotary) {
+              const float2 w = turn[(x.d0 + i) >> 1];
+              const float f = a[i], g = a[i + 1];
+              a[i] = f * w.x - g * w.y;
+              a[i + 1] = g * w.x + f * w.y;
+            }
+            if (x.d1 + i < p.rotary) {
+              const float2 w = turn[(x.d1 + i) >> 1];
+              const float f = b[i], g = b[i + 1];
+              b[i] = f * w.x - g * w.y;
+              b[i + 1] = g * w.x + f * w.y;
+            }
+          }
+        }
+      }
+      if (F8 && x.cached) {
+        uint8_t *codes = reinterpret_cast<uint8_t *>(x.dst);
+        store_e4m3<VEC, ALIGNED>(codes + x.d0, a, x.scale);
+        if (both) store_e4m3<VEC, ALIGNED>(codes + x.d1, b, x.scale);
+        continue;
+      }
+      ca = pack<BF16, VEC>(a);
+      cb = pack<BF16, VEC>(b);
+    }
+    store<VEC, ALIGNED>(x.dst + x.d0, ca);
+    if (both) store<VEC, ALIGNED>(x.dst + x.d1, cb);
+  }
+}
+
+template <bool BF16, bool F8>
+void launch(const AppendParams &p, int vec, bool aligned, unsigned blocks, cudaStream_t stream) {
+  if (vec == 8) append_kernel<BF16, F8, 8, true><<<blocks, kAppendThreads, 0, stream>>>(p);
+  else if (vec == 4) append_kernel<BF16, F8, 4, true><<<blocks, kAppendThreads, 0, stream>>>(p);
+  else if (vec == 2) append_kernel<BF16, F8, 2, false><<<blocks, kAppendThreads, 0, stream>>>(p);
+  else append_kernel<BF16, F8, 1, false><<<blocks, kAppendThreads, 0, stream>>>(p);
+  GCB_CUDA(cudaGetLastError());
+  count_launch();
+}
+
+void require(bool ok, const char *what) {
+  if (!ok) throw std::invalid_argument(what);
+}
+
+} // namespace
+
+PagedCache checked_cache(const gcb200_paged_cache &c, bool writes) {
+  require(c.dtype == GCB200_BF16 || c.dtype == GCB200_F16, "paged cache: dtype must be bf16 or f16");
+  require(c.cache_dtype == c.dtype || c.cache_dtype == GCB200_F8_E4M3, "paged cache: the cache must have the operands' type, or e4m3");
+  require(c.keys && c.values && (c.page_table || c.sequences == 0 || c.max_pages == 0), "paged cache: null pointer");
+  require(c.pages > 0 && c.page_size > 0 && c.kv_heads > 0 && c.sequences >= 0 && c.max_pages >= 0, "paged cache: sizes must be positive");
+  require(c.pages < (int64_t(1) << 31) && c.sequences < (int64_t(1) << 31) && c.kv_heads < 65536 && c.page_size <= (int64_t(1) << 30) &&
+              c.max_pages < (int64_t(1) << 31) && c.page_size * c.max_pages < (int64_t(1) << 31),
+          "paged cache: positions and page numbers are 32-bit");
+  const int size = c.cache_dtype == GCB200_F8_E4M3 ? 1 : 2;
+  require(c.head_dim >= 8 && c.head_dim <= kMaxDim && c.head_dim * size % 16 == 0,
+          "paged cache: head_dim must be at most 256 and a multiple of 8 (of 16 for an 8-bit cache)");
+  require(size == 1 || (!c.key_scale && !c.value_scale), "paged cache: scales are for 8-bit caches");
+  require(c.sequences <= 1 || c.page_table_stride >= c.max_pages, "paged cache: rows of the page table overlap");
+  const int64_t extent[3] = {c.pages, c.kv_heads, c.page_size};
+  int64_t ks[3], vs[3];
+  for (int i = 0; i < 3; ++i) {
+    // the stride of a dimension of one is never used, whatever it says
+    ks[i] = extent[i] > 1 ? c.key_stride[i] * size : 0;
+    vs[i] = extent[i] > 1 ? c.value_stride[i] * size : 0;
+    require(ks[i] >= 0 && vs[i] >= 0 && ks[i] % 16 == 0 && vs[i] % 16 == 0, "paged cache: strides must be multiples of 16 bytes");
+    if (writes && extent[i] > 1) require(ks[i] >= c.head_dim * size && vs[i] >= c.head_dim * size, "paged cache: rows of the cache overlap");
+  }
+  require(((reinterpret_cast<uintptr_t>(c.keys) | reinterpret_cast<uintptr_t>(c.values)) & 15) == 0, "paged cache: keys and values must be 16-byte aligned");
+  PagedCache d{};
+  d.keys = static_cast<uint8_t *>(c.keys);
+  d.values = static_cast<uint8_t *>(c.values);
+  d.key_page = ks[0]; d.key_head = ks[1]; d.key_token = ks[2];
+  d.value_page = vs[0]; d.value_head = vs[1]; d.value_token = vs[2];
+  d.key_scale = c.key_scale;
+  d.value_scale = c.value_scale;
+  d.table = PageTable{c.page_table, c.page_table_stride, int(c.sequences), int(c.max_pages), int(c.page_size), int(c.pages)};
+  d.kv_heads = int(c.kv_heads);
+  d.dim = int(c.head_dim);
+  return d;
+}
+
+void paged_kv_append(const gcb200_paged_cache &cache, const AppendArgs &a, cudaStream_t stream) {
+  AppendParams p{};
+  p.c = checked_cache(cache, true);
+  require(a.tokens == 0 || (a.k && a.v && a.positions), "paged append: null pointer");
+  require(!a.q || a.q_out, "paged append: queries without a place to go");
+  require(a.tokens >= 0 && a.tokens < (int64_t(1) << 31), "paged append: number of tokens out of range");
+  require(!a.q || (a.heads > 0 && a.heads < 65536), "paged append: number of heads out of range");
+  require(a.sequences || a.tokens <= cache.sequences, "paged append: more tokens than sequences, and no sequence numbers");
+  require(a.inv_freq ? a.rotary_dim >= 2 && a.rotary_dim % 2 == 0 && a.rotary_dim <= cache.head_dim : a.rotary_dim == 0,
+          "paged append: rotary_dim must be even and at most head_dim (0 without inv_freq)");
+  if (a.tokens == 0) return;
+  DeviceState &dev = device_state();
+  p.c.error = dev.d_error;
+  p.q = static_cast<const uint16_t *>(a.q);
+  p.k = static_cast<const uint16_t *>(a.k);
+  p.v = static_cast<const uint16_t *>(a.v);
+  p.q_out = static_cast<uint16_t *>(a.q_out);
+  auto of = [](const int64_t s[2], int64_t tokens, int64_t heads, int64_t &token, int64_t &head) {
+    token = tokens > 1 ? s[0] : 0;
+    head = heads > 1 ? s[1] : 0;
+  };
+  if (a.q) {
+    of(a.q_stride, a.tokens, a.heads, p.q_token, p.q_head);
+    of(a.q_out_stride, a.tokens, a.heads, p.o_token, p.o_head);
+  }
+  of(a.k_stride, a.tokens, cache.kv_heads, p.k_token, p.k_head);
+  of(a.v_stride, a.tokens, cache.kv_heads, p.v_token, p.v_head);
+  p.sequences = a.sequences;
+  p.positions = a.positions;
+  p.inv_freq = a.inv_freq;
+  p.heads = int(a.heads);
+  p.rotary = int(a.rotary_dim);
+  p.interleaved = a.interleaved;
+  // the widest chunk that every address and both halves of a rotation are multiples of
+  const int64_t rest = cache.head_dim - a.rotary_dim, half = a.rotary_dim / 2;
+  int64_t all = int64_t(reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) | 2 * (p.k_token | p.k_head | p.v_token | p.v_head);
+  if (a.q) all |= int64_t(reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.q_out)) | 2 * (p.q_token | p.q_head | p.o_token | p.o_head);
+  const int64_t pieces = a.interleaved ? 0 : (half | rest);
+  int vec = all % 16 == 0 && pieces % 8 == 0 ? 8 : all % 8 == 0 && pieces % 4 == 0 ? 4 : pieces % 2 == 0 ? 2 : 1;
+  const int64_t chunks = cache.head_dim / vec;
+  const int64_t rotated_units = a.interleaved || !a.rotary_dim ? 0 : half / vec + (rest / vec + 1) / 2;
+  p.units = int(std::max((chunks + 1) / 2, rotated_units));
+  const bool bf16 = cache.dtype == GCB200_BF16, f8 = cache.cache_dtype == GCB200_F8_E4M3;
+  (bf16 ? (f8 ? launch<true, true> : launch<true, false>) : (f8 ? launch<false, true> : launch<false, false>))(p, vec, vec >= 4, unsigned(a.tokens), stream);
+}
+
+} // namespace gcb

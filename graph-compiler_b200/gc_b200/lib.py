@@ -43,6 +43,14 @@ class TpMlpDesc(C.Structure):
                 ("recv_planes", _int)]
 
 
+class PagedCacheDesc(C.Structure):
+    """Mirror of ``gcb200_paged_cache``."""
+
+    _fields_ = [("dtype", _int), ("cache_dtype", _int), ("pages", _i64), ("page_size", _i64), ("kv_heads", _i64), ("head_dim", _i64),
+                ("keys", _vp), ("values", _vp), ("key_stride", _i64 * 3), ("value_stride", _i64 * 3), ("key_scale", _vp), ("value_scale", _vp),
+                ("page_table", _vp), ("sequences", _i64), ("max_pages", _i64), ("page_table_stride", _i64)]
+
+
 _lib = None
 
 
@@ -93,6 +101,14 @@ def load() -> C.CDLL:
         "gcb200_tp_mlp_timeline": [_vp, _vp, _vp, C.c_char_p, C.c_size_t, C.POINTER(C.c_size_t)],
         "gcb200_tp_mlp_trace": [_vp, C.c_char_p, C.c_size_t, C.POINTER(C.c_size_t)],
         "gcb200_wait_selftest": [C.c_longlong, _vp],
+        "gcb200_paged_kv_append": [C.POINTER(PagedCacheDesc), _vp, C.POINTER(_i64), _i64, _vp, C.POINTER(_i64), _vp, C.POINTER(_i64), _vp,
+                                   C.POINTER(_i64), _vp, _vp, _i64, _vp, _i64, _int, _vp],
+        "gcb200_paged_attention_workspace": [_i64, _i64, _i64, C.POINTER(C.c_size_t)],
+        "gcb200_paged_attention": [C.POINTER(PagedCacheDesc), _vp, C.POINTER(_i64), _i64, _vp, _f32, _i64, _vp, C.POINTER(_i64), _vp, _vp,
+                                   C.c_size_t, _vp],
+        "gcb200_w4_packed_bytes": [_i64, _i64, _i64, _int, C.POINTER(C.c_size_t)],
+        "gcb200_w4_pack": [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp],
+        "gcb200_matmul_w4": [_int, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int, _int, _vp],
     }
     for name, argtypes in sig.items():
         fn = getattr(lib, name)
@@ -139,6 +155,7 @@ def host():
     if torch is not None:
         _host_module.setup(torch.Tensor, torch.bfloat16, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream,
                            _ndarray())
+        _host_module.types(torch.float16, torch.float8_e4m3fn, torch.int32, torch.float32, torch.float64, torch.uint8)
         _host = _host_module
     return _host_module
 
@@ -382,6 +399,116 @@ def attention_bf16(Q, K, V, scale: float, causal: bool = False, out=None):
     if out is None:
         out = torch.empty_like(Q)
     check(load().gcb200_attention_bf16(_ptr(Q), _ptr(K), _ptr(V), _ptr(out), bh, S, D, float(scale), int(causal), _stream()))
+    return out
+
+
+# ----------------------------------------------------------------------------- decode over a paged key-value cache
+def paged_kv_append(q, k, v, key_cache, value_cache, page_table, positions, sequences=None, inv_freq=None, interleaved=False,
+                    key_scale=None, value_scale=None, out=None):
+    """Writes new keys and values, rotated by their positions, into their pages; returns the rotated queries (``None`` without q).
+
+    q ``[tokens, heads, dim]`` (or None), k and v ``[tokens, kv_heads, dim]``, bf16 or f16, any strides before the last dimension.
+    Caches ``[pages, kv_heads, page_size, dim]`` of the same type, or float8_e4m3fn with ``key_scale`` / ``value_scale`` (f32
+    ``[kv_heads]``); a cache stored ``[pages, page_size, kv_heads, dim]`` is passed as its ``transpose(1, 2)``.
+    ``page_table`` int32 ``[sequences, pages of a sequence]``, ``positions`` int32 ``[tokens]``, ``sequences`` int32 ``[tokens]``
+    (None: token t belongs to sequence t).  A negative sequence or position marks padding, whose rows stay as they are.
+    ``inv_freq`` float64 ``[rotary_dim / 2]`` (None: no rotation); ``interleaved``: pairs (2 i, 2 i + 1) instead of halves.
+    ``out`` may be q itself.  Pages outside the cache are not written; :func:`device_error` then gives 9."""
+    if q is not None and out is None:
+        import torch
+
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    st = (_host or host()).paged_kv_append(q, k, v, key_cache, value_cache, page_table, positions, sequences, inv_freq, interleaved,
+                                           key_scale, value_scale, out)
+    if st:
+        check(st)
+    return out if q is not None else None
+
+
+_workspace_bytes: dict = {}
+
+
+def paged_attention_workspace(q, key_cache):
+    """Scratch memory for :func:`paged_attention` calls with these heads, one after another on one stream."""
+    import torch
+
+    assert q.is_cuda and q.dim() == 3 and key_cache.dim() == 4, "q must be [sequences, heads, dim] on a CUDA device, the cache [pages, kv_heads, page_size, dim]"
+    key = (q.device, q.shape[1], key_cache.shape[1], q.shape[2])
+    n = _workspace_bytes.get(key)
+    if n is None:
+        size = C.c_size_t(0)
+        with torch.cuda.device(q.device):
+            check(load().gcb200_paged_attention_workspace(q.shape[1], key_cache.shape[1], q.shape[2], C.byref(size)))
+        n = _workspace_bytes[key] = size.value
+    return torch.empty(n, dtype=torch.uint8, device=q.device)
+
+
+def paged_attention(q, key_cache, value_cache, page_table, lengths, scale: float, window: int = 0, key_scale=None, value_scale=None,
+                    out=None, lse=None, workspace=None):
+    """Attention of one new token per sequence over its cached tokens (:func:`paged_kv_append` describes the cache).
+
+    q ``[sequences, heads, dim]``; heads a multiple of the cache's, query head h reads KV head ``h // (heads // kv_heads)``.
+    ``lengths`` int32 ``[sequences]``: tokens in the cache, the new one among them; 0 gives zeros.  ``window`` > 0: the last
+    ``window`` tokens only.  ``lse`` f32 ``[sequences, heads]`` receives the logarithm of the softmax's sum (-inf for length 0).
+    ``workspace``: what :func:`paged_attention_workspace` gave, kept by the caller and used by one call at a time; by default
+    each call takes its own from torch's allocator."""
+    if out is None:
+        import torch
+
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if workspace is None:
+        workspace = paged_attention_workspace(q, key_cache)
+    st = (_host or host()).paged_attention(q, key_cache, value_cache, page_table, lengths, scale, window, key_scale, value_scale, out, lse,
+                                           workspace)
+    if st:
+        check(st)
+    return out
+
+
+# ----------------------------------------------------------------------------- 4-bit weights
+class W4Weights:
+    """Packed 4-bit weights of one linear layer (:func:`pack_w4`): N outputs, K inputs, one scale (and zero) per ``group`` inputs."""
+
+    __slots__ = ("packed", "N", "K", "group", "has_zeros", "dtype")
+
+    def __init__(self, packed, N, K, group, has_zeros, dtype):
+        self.packed, self.N, self.K, self.group, self.has_zeros, self.dtype = packed, N, K, group, has_zeros, dtype
+
+
+def pack_w4(codes, scales, K: int, group: int, zeros=None) -> W4Weights:
+    """Lays 4-bit weights out for :func:`matmul_w4`, once: W[n, k] = (code - zero) * scale.
+
+    ``codes`` uint8 ``[N, (K + 1) // 2]``, even k in the low half of a byte; ``scales`` bf16 or f16 ``[N, ceil(K / group)]``;
+    ``zeros`` uint8 ``[N, ceil(K / group)]`` of 0..15 (None: 8).  ``group`` is 32, 64 or a multiple of 128."""
+    import torch
+
+    N = codes.shape[0]
+    need = C.c_size_t(0)
+    check(load().gcb200_w4_packed_bytes(N, K, group, int(zeros is not None), C.byref(need)))
+    groups = -(-K // group)
+    assert codes.dtype == torch.uint8 and tuple(codes.shape) == (N, (K + 1) // 2), "codes must be uint8 [N, (K + 1) // 2]"
+    assert scales.dtype in (torch.bfloat16, torch.float16) and tuple(scales.shape) == (N, groups), "scales must be bf16 or f16 [N, ceil(K / group)]"
+    assert zeros is None or (zeros.dtype == torch.uint8 and tuple(zeros.shape) == (N, groups)), "zeros must be uint8 [N, ceil(K / group)]"
+    for t in (codes, scales, zeros):
+        if t is not None:
+            assert t.is_cuda and t.get_device() == torch.cuda.current_device(), "the weights must be on the current CUDA device"
+            assert t.shape[1] == 1 or t.stride(1) == 1, "the weights must be contiguous in their last dimension"
+    packed = torch.empty(need.value, dtype=torch.uint8, device=codes.device)
+    check(load().gcb200_w4_pack(_ptr(codes), codes.stride(0), _ptr(scales), scales.stride(0), _ptr(zeros), 0 if zeros is None else zeros.stride(0),
+                                N, K, group, _ptr(packed), _stream()))
+    return W4Weights(packed, N, K, group, zeros is not None, scales.dtype)
+
+
+def matmul_w4(x, weights: W4Weights, bias=None, relu: bool = False, out=None):
+    """act(x . W^T + bias) for a few rows: x ``[M, K]`` of the scales' type, f32 products and sums, rounded once."""
+    w = weights
+    if out is None:
+        import torch
+
+        out = torch.empty((x.shape[0], w.N), dtype=x.dtype, device=x.device)
+    st = (_host or host()).matmul_w4(x, w.packed, w.dtype, w.N, w.K, w.group, w.has_zeros, bias, relu, out)
+    if st:
+        check(st)
     return out
 
 

@@ -196,6 +196,71 @@ int gcb200_attention_bf16(const void *Q, const void *K, const void *V, void *O, 
                           int64_t head_dim, float scale, int causal, void *stream);
 
 /* ---------------------------------------------------------------------------
+ * Decode over a paged key-value cache (extension: the reference computes attention from matmul and softmax pieces over
+ * whole K and V tensors, lib/gc/Transforms/DecomposeAggregatedOps.cpp:24-38, and keeps no cache).
+ *
+ * Keys and values lie in pages of `page_size` tokens: keys + page * key_stride[0] + kv_head * key_stride[1] +
+ * (position % page_size) * key_stride[2], head_dim contiguous elements each; strides are in elements, so heads may lie
+ * outside tokens or tokens outside heads.  Row `s` of page_table holds the pages of sequence s in the order of its positions;
+ * entries behind its last token are not read.  head_dim is a multiple of 8 (of 16 for 8-bit caches), at most 256; the
+ * caches' base addresses and strides are multiples of 16 bytes.  cache_dtype is dtype, or GCB200_F8_E4M3: a cached number is
+ * then code * scale of its KV head.  A page number outside [0, pages) that a call meets is never followed: the call records
+ * code 9 in the device error word (gcb200_device_error), and those tokens count as zeros (attention) or are not written
+ * (append). */
+typedef enum { GCB200_F16 = 1, GCB200_BF16 = 2, GCB200_F8_E4M3 = 10 } gcb200_dtype; /* dnnl_data_type_t's codes where it has one */
+typedef struct {
+  int dtype;                      /* queries, new keys and values, results: GCB200_BF16 or GCB200_F16 */
+  int cache_dtype;
+  int64_t pages, page_size, kv_heads, head_dim;
+  void *keys, *values;
+  int64_t key_stride[3], value_stride[3];   /* elements between pages, between heads, between tokens */
+  const float *key_scale, *value_scale;     /* [kv_heads], positive; 8-bit caches only (NULL: 1) */
+  const int32_t *page_table;                /* [sequences] rows of max_pages, page_table_stride elements apart */
+  int64_t sequences, max_pages, page_table_stride;
+} gcb200_paged_cache;
+
+/* Appends new keys and values, rotated by their positions on the way, and rotates the queries that belong to them.
+ * Token t belongs to sequence sequences[t] (NULL: to sequence t) and stands at positions[t].  With inv_freq (device, f64,
+ * rotary_dim / 2 of them; NULL: no rotation) pair i of the first rotary_dim elements of a query or key turns by the angle
+ * positions[t] * inv_freq[i], which is formed and reduced in 64 bits; a pair is (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when
+ * interleaved.  The rotation is computed in f32 and rounded once; 8-bit caches hold round(x / scale), limited to +-448.
+ * q [tokens][heads][head_dim] (may be NULL) goes to q_out, which may be q itself; strides (elements) are those of tokens and heads;
+ * k and v have kv_heads.  A token with a negative sequence or position is padding: its queries are left out too.
+ * No two tokens of a call may share a sequence and a position, and no two sequences a page that either appends to. */
+int gcb200_paged_kv_append(const gcb200_paged_cache *cache, const void *q, const int64_t q_stride[2], int64_t heads,
+                           const void *k, const int64_t k_stride[2], const void *v, const int64_t v_stride[2], void *q_out,
+                           const int64_t q_out_stride[2], const int32_t *sequences, const int32_t *positions, int64_t tokens,
+                           const double *inv_freq, int64_t rotary_dim, int interleaved, void *stream);
+
+/* Attention of one new token per sequence: out[s][h] = sum_t softmax_t(scale * q[s][h] . k_t) v_t over the positions t in
+ * [max(0, lengths[s] - window), lengths[s]) of sequence s (window 0: all), keys and values of KV head h / (heads / kv_heads).
+ * lengths (device) count the tokens in the cache, the new one among them.  A sequence of length 0 (or less) gives zeros, and
+ * minus infinity in lse.  lse [sequences][heads] f32 (may be NULL) receives log sum_t exp(scale * q . k_t).  Scores, maxima, sums
+ * and results are held in f32; exp() of the scores is rounded to 16 bits (like the values it multiplies) and the result once.
+ * A length beyond max_pages * page_size is cut to that and recorded as code 9 in the device error word.
+ * workspace: device memory, gcb200_paged_attention_workspace() bytes, 16-byte aligned, that no other call in flight uses; nothing
+ * in it needs clearing or is kept from one call to the next. */
+int gcb200_paged_attention_workspace(int64_t heads, int64_t kv_heads, int64_t head_dim, size_t *bytes);
+int gcb200_paged_attention(const gcb200_paged_cache *cache, const void *q, const int64_t q_stride[2], int64_t heads,
+                           const int32_t *lengths, float scale, int64_t window, void *out, const int64_t out_stride[2],
+                           float *lse, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Few rows against 4-bit weights (extension of the u8 x s8 path's per-channel scales to groups along K):
+ *
+ *   Y = act( X . W^T + bias ),   W[n][k] = (code[n][k] - zero[n][k / group]) * scale[n][k / group],  codes and zeros 0..15
+ * X [M][K], Y [M][N], bias [N] and the scales are `dtype` (bf16 or f16); products and sums are f32, rounded once.
+ * group is 32, 64 or a multiple of 128.  gcb200_w4_pack lays the weights out once, in the order in which the kernel reads them:
+ * codes [N] rows of (K + 1) / 2 bytes (even k in the low half of a byte), scales and zeros [N][ceil(K / group)] (zeros NULL: 8);
+ * row strides are in elements.  packed: gcb200_w4_packed_bytes() bytes, 16-byte aligned.  The scales' type is that of the X the
+ * weights will meet.  Any M; more than 16 rows read the weights once for every 16. */
+int gcb200_w4_packed_bytes(int64_t N, int64_t K, int64_t group, int has_zeros, size_t *bytes);
+int gcb200_w4_pack(const uint8_t *codes, int64_t codes_stride, const void *scales, int64_t scales_stride, const uint8_t *zeros,
+                   int64_t zeros_stride, int64_t N, int64_t K, int64_t group, void *packed, void *stream);
+int gcb200_matmul_w4(int dtype, const void *X, int64_t ldx, const void *packed, const void *bias, void *Y, int64_t ldy, int64_t M,
+                     int64_t N, int64_t K, int64_t group, int has_zeros, int relu, void *stream);
+
+/* ---------------------------------------------------------------------------
  * Additions around the dnnl_graph_compiler_* API (declared in
  * dnnl_graph_compiler.h; tensor struct repeated here as an opaque pointer to
  * keep this header standalone).
