@@ -1,8 +1,25 @@
 // Attention of one new token per sequence over a paged key-value cache:
-//   out = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale q . k_t - m),  m = max_t scale q . k_t
-// with the running maximum and sum of an online softmax, so that keys and values are read once.
+//   out = sum_t p_t v_t / sum_t p_t,  p_t = 2^(x_t - m),  x_t = log2(e) scale q . k_t,  m a reference close to max_t x_t
+// with the running reference and sum of an online softmax, so that keys and values are read once.
 //
-// Bound by HBM: 2 head_dim elements of cache per token and KV head for 4 head_dim operations per query head.
+// Bound by HBM: 2 head_dim elements of cache per token and KV head, for 4 head_dim operations per query head, so everything is
+// arranged for an even, unbroken stream of the cache:
+//  * Work.  Sequences have any length, and the host does not know it (a captured step follows lengths in device memory).  Every
+//    block adds up the lengths itself and takes an equal share of all tiles of tokens (paged_index.h).  Units (a sequence's KV
+//    head) that a border cuts leave f32 parts in the workspace, which a second kernel, started behind the first by a dependent
+//    launch, joins in the order of the blocks: the same bits every time, and no counter that a call leaves behind.
+//  * A warp fetches its own tokens (16 or 32 of a tile) with asynchronous 16-byte copies, three tiles ahead, and waits for nobody:
+//    page numbers come one tile further ahead, so that no copy waits for the table.  Rows behind the sequence's end are filled with
+//    zeros by the copy.
+//  * Products on the tensor cores with the TOKENS on the instruction's 16-row side and the query heads of the KV head on its
+//    8-column side: S^T = K Q^T and O^T += V^T P^T.  Eight heads to a KV head fill it; fewer leave columns empty, which costs
+//    nothing that the stream would notice.  P^T goes from the result layout of the first product to the operand layout of the
+//    second by an 8 x 8 transposition in registers.
+//  * The reference m only follows the maximum when that has grown by more than 2^8: one vote per tile instead of a reduction.
+//  * P is rounded once to the type of the product (a second product with the rounding's rest would halve the error, and turn an
+//    infinite value into NaN).  In f16 the reference lies 2^7 below the maximum: without that, tokens below 2^-25 of the largest
+//    would vanish, and a hundred thousand of them may hold a third of a percent of the sum.
+//  * 8-bit caches become f16 in registers (exact).  Queries are scaled to f16 by a power of two per head.
 #include "decode_ops.h"
 
 #include <algorithm>
@@ -17,6 +34,10 @@ namespace gcb {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kStages = 3;
+constexpr int kMaxBlocks = 592;   // the workspace has two parts for each
+constexpr float kLazy = 8.f;
 
 struct PagedAttParams {
   PagedCache c;
@@ -24,90 +45,584 @@ struct PagedAttParams {
   uint16_t *out;
   int64_t q_seq, q_head, o_seq, o_head;   // elements
   const int32_t *lengths;
-  float *lse;
-  float scale;
-  int heads, group, window;
+  float *lse, *parts;
+  float scale_log2e;
+  int heads, group, sets, window, blocks, least;   // sets: of query heads per KV head, each the columns of one product
+  bool q_aligned, same_strides;
 };
 
-template <bool BF16, bool F8> __device__ __forceinline__ void load8(const uint8_t *p, float (&x)[8]) {
-  if constexpr (F8) {
-    const uint2 u = *reinterpret_cast<const uint2 *>(p);
-    const uint32_t w[2] = {u.x, u.y};
+// What a template instance keeps in shared memory.
+template <bool F8, int DP, int NT> struct Shape {
+  static constexpr int kRow = DP * (F8 ? 1 : 2);            // bytes of a token's row
+  static constexpr int kChunks = kRow / 16;
+  static constexpr int kTokens = kRow <= 128 ? 32 : 16;     // of a warp in a tile
+  static constexpr int kTile = kWarps * kTokens;
+  static constexpr int kSlot = 2 * kTokens * kRow;          // a warp's keys and values of one tile
+  static constexpr int kCols = 8 * NT;                      // query heads
+  static constexpr int kQRow = DP * 2 + 16;                 // bytes, padded against bank conflicts
+  static constexpr int kQ = kCols * kQRow;
+  static constexpr int kBytes = kStages * kWarps * kSlot + (kStages + 1) * kQ;
+  static_assert(kCols * DP * 4 <= kSlot, "a warp's results fit where its tokens were");
+};
+// Part of a cut unit in the workspace: [cols][dim] f32 sums, then m and l of each column.
+__host__ __device__ __forceinline__ int64_t part_floats(int cols, int dim) { return int64_t(cols) * (dim + 2); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }   // -inf - -inf would be NaN
+
+// Where tile number `want` of the row of all tiles is: its sequence, the tiles of that sequence's units, and the tile's number from
+// the first tile of the sequence.  All threads of the block call it; pre has room for kThreads + 1.
+struct Place {
+  int seq;
+  int64_t rest;     // tiles between the sequence's first and `want`
+};
+template <int TILE> __device__ __forceinline__ int64_t count_tiles(const PagedAttParams &p, int units, int64_t *pre) {
+  const int n = p.c.table.sequences, each = (n + kThreads - 1) / kThreads, s0 = threadIdx.x * each, s1 = min(n, s0 + each);
+  int64_t mine = 0;
+  for (int s = s0; s < s1; ++s) mine += tiles_of(seen_of(p.c.table, p.lengths[s], p.window), TILE);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t sum = mine;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t h = e4m3x2_to_f16x2((w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
-      x[2 * i] = half_to_f32<false>(h & 0xFFFFu);
-      x[2 * i + 1] = half_to_f32<false>(h >> 16);
-    }
-  } else {
-    const uint4 u = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  for (int i = 1; i < 32; i <<= 1) {
+    const int64_t other = __shfl_up_sync(0xFFFFFFFFu, sum, i);
+    if (lane >= i) sum += other;
+  }
+  __shared__ int64_t warp_sum[kWarps];
+  if (lane == 31) warp_sum[warp] = sum;
+  __syncthreads();
+  int64_t before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = half_to_f32<BF16>(w[i] & 0xFFFFu);
-      x[2 * i + 1] = half_to_f32<BF16>(w[i] >> 16);
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += warp_sum[w];
+    all += warp_sum[w];
+  }
+  pre[threadIdx.x] = before + sum - mine;
+  if (threadIdx.x == 0) pre[kThreads] = all;
+  return all * units;
+}
+// Behind count_tiles; `want` < total.  `found` is shared.
+template <int TILE> __device__ __forceinline__ Place locate(const PagedAttParams &p, int units, const int64_t *pre, int64_t want, Place *found) {
+  if (threadIdx.x == 0) *found = Place{};
+  __syncthreads();
+  const int n = p.c.table.sequences, each = (n + kThreads - 1) / kThreads;
+  int64_t at = pre[threadIdx.x] * units;
+  if (at <= want && want < pre[threadIdx.x + 1] * units) {
+    int s = threadIdx.x * each;
+    for (; s < n - 1; ++s) {
+      const int64_t here = int64_t(tiles_of(seen_of(p.c.table, p.lengths[s], p.window), TILE)) * units;
+      if (want < at + here) break;
+      at += here;
     }
+    found->seq = s;
+    found->rest = want - at;
+  }
+  __syncthreads();
+  return *found;
+}
+
+// Walks the row of tiles.
+struct Cursor {
+  int seq, unit, tile, tiles, first, end;
+};
+template <int TILE> __device__ __forceinline__ void open_sequence(const PagedAttParams &p, Cursor &c) {
+  const Seen s = seen_of(p.c.table, p.lengths[c.seq], p.window);
+  c.first = s.first;
+  c.end = s.end;
+  c.tiles = tiles_of(s, TILE);
+}
+// To the next tile, which must exist.
+template <int TILE> __device__ __forceinline__ void advance(const PagedAttParams &p, int units, Cursor &c) {
+  if (++c.tile < c.tiles) return;
+  c.tile = 0;
+  if (++c.unit < units) return;
+  c.unit = 0;
+  do {
+    if (c.seq + 1 >= p.c.table.sequences) return;   // only if somebody changes the lengths meanwhile
+    ++c.seq;
+    open_sequence<TILE>(p, c);
+  } while (c.tiles == 0);
+}
+
+// 16-byte chunk `ch` of row `r`: chunks of eight neighbouring rows lie in different banks.
+template <int CHUNKS> __device__ __forceinline__ uint32_t chunk_at(int r, int ch) {
+  if constexpr (CHUNKS >= 8) return uint32_t(r * CHUNKS + (ch ^ (r & 7))) * 16u;
+  else return uint32_t(r * CHUNKS + (ch ^ ((r >> 1) & 3))) * 16u;
+}
+
+template <bool BF16, bool F8, int DP, int NT>
+__global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_constant__ PagedAttParams p) {
+  using S = Shape<F8, DP, NT>;
+  constexpr bool kMmaBf16 = BF16 && !F8;
+  constexpr int kSteps = DP / 16, kSubs = S::kTokens / 16;
+  constexpr float kBelow = kMmaBf16 ? 0.f : 7.f;   // the reference under the maximum: P reaches 2^(kBelow + kLazy), below f16's 2^16
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int64_t pre[kThreads + 1];
+  __shared__ Place found;
+  __shared__ float stat_m[kWarps][S::kCols], stat_l[kWarps][S::kCols];
+
+  const PagedCache &c = p.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row8 = lane >> 2, col4 = lane & 3;
+  const int units = c.kv_heads * p.sets, dim = c.dim;
+  pdl_wait();
+  pdl_launch_dependents();   // behind the wait: what starts now finds everything before this kernel done
+
+  const int64_t total = count_tiles<S::kTile>(p, units, pre), per = share_of(total, p.blocks, p.least);
+  const int64_t begin = int64_t(blockIdx.x) * per, stop = min(total, begin + per);
+
+  if (begin < stop) {
+    Place at = locate<S::kTile>(p, units, pre, begin, &found);
+    Cursor comp;   // of the tile being computed
+    comp.seq = at.seq;
+    open_sequence<S::kTile>(p, comp);
+    comp.unit = min(units - 1, int(at.rest / max(1, comp.tiles)));
+    comp.tile = int(at.rest - int64_t(comp.unit) * comp.tiles);
+    Cursor ahead = comp;   // of the tile whose page numbers are being fetched
+    const int count = int(stop - begin);
+    const int first_tile = comp.tile;
+
+    uint8_t *mine = smem + warp * kStages * S::kSlot;
+    uint8_t *qring = smem + kWarps * kStages * S::kSlot;
+    // ---- what the next tile to fetch needs: this lane's token's page and slot
+    int next_page = -1, next_slot = 0, next_seq = 0, next_unit = 0, fetched = 0, segments = 0;
+    bool next_new = true;
+    auto look_up = [&]() {
+      next_seq = ahead.seq;
+      next_unit = ahead.unit;
+      next_new = fetched == 0 || ahead.tile == 0;
+      const int pos = ahead.first + ahead.tile * S::kTile + warp * S::kTokens + lane;
+      next_page = -1;
+      next_slot = 0;
+      if (lane < S::kTokens && pos < ahead.end) {
+        next_page = page_of(c.table, ahead.seq, pos);
+        next_slot = pos % c.table.page_size;
+        if (next_page < 0) atomicExch(c.error, int(ERR_BAD_PAGE));
+      }
+      if (++fetched < count) advance<S::kTile>(p, units, ahead);
+    };
+    const int lane_row = lane / S::kChunks, lane_chunk = lane % S::kChunks;
+    const bool lane_copies = lane_chunk * 16 < dim * (F8 ? 1 : 2);
+    auto issue = [&](int stage) {
+      const int kv = next_unit / p.sets, set = next_unit - kv * p.sets;
+      if (next_new) {
+        uint8_t *dst = qring + (segments % (kStages + 1)) * S::kQ;
+        ++segments;
+        for (int i = threadIdx.x; i < S::kCols * (DP / 8); i += kThreads) {
+          const int col = i / (DP / 8), d = (i - col * (DP / 8)) * 8, in_group = set * S::kCols + col;
+          const bool there = in_group < p.group && d < dim;
+          const uint16_t *src = p.q + (there ? next_seq * p.q_seq + (kv * p.group + in_group) * p.q_head + d : 0);
+          uint8_t *to = dst + col * S::kQRow + d * 2;
+          if (p.q_aligned) {
+            cp_async_16(smem_u32(to), src, there ? 16u : 0u);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) reinterpret_cast<uint16_t *>(to)[e] = there ? src[e] : uint16_t(0);
+          }
+        }
+      }
+      const int64_t koff = next_page < 0 ? -1 : next_page * c.key_page + next_slot * c.key_token;
+      const int64_t voff = p.same_strides || next_page < 0 ? koff : next_page * c.value_page + next_slot * c.value_token;
+      const uint8_t *kbase = c.keys + kv * c.key_head + lane_chunk * 16, *vbase = c.values + kv * c.value_head + lane_chunk * 16;
+      const uint32_t dst = smem_u32(mine + stage * S::kSlot);
+#pragma unroll
+      for (int i = 0; i < S::kTokens * S::kChunks / 32; ++i) {
+        const int r = i * (32 / S::kChunks) + lane_row;
+        const int64_t ko = __shfl_sync(0xFFFFFFFFu, koff, r);
+        const int64_t vo = p.same_strides ? ko : __shfl_sync(0xFFFFFFFFu, voff, r);
+        if (lane_copies) {
+          const uint32_t to = dst + chunk_at<S::kChunks>(r, lane_chunk), bytes = ko < 0 ? 0u : 16u;
+          cp_async_16(to, kbase + (ko < 0 ? 0 : ko), bytes);
+          cp_async_16(to + S::kTokens * S::kRow, vbase + (ko < 0 ? 0 : vo), bytes);
+        }
+      }
+      look_up();
+    };
+
+    look_up();
+    for (int i = 0; i < kStages; ++i) {
+      if (i < count) issue(i);
+      cp_async_commit();
+    }
+
+    uint32_t qf[kSteps][NT][2];
+    float acc[kSteps][NT][4], m[NT][2], l[NT][2], factor[NT][2];
+    int stage = 0, segment = 0;
+    bool fresh = true;   // the tile is the first one of its unit here
+    for (int x = 0; x < count; ++x) {
+      cp_async_wait<kStages - 1>();
+      __syncwarp();
+      if (fresh) {
+        __syncthreads();   // the queries were fetched by all warps
+        const uint8_t *qs = qring + (segment % (kStages + 1)) * S::kQ + row8 * S::kQRow;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint8_t *qrow = qs + n * 8 * S::kQRow;
+          float mul = p.scale_log2e;
+          if constexpr (F8) {
+            // a power of two brings the row's largest magnitude to [2^7, 2^8); what f16 then drops is below 2^-31 of it
+            float big = 0.f;
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+              const uint2 u = *reinterpret_cast<const uint2 *>(qrow + j * 32 + col4 * 8);
+              big = fmaxf(big, fmaxf(fmaxf(fabsf(half_to_f32<BF16>(u.x & 0xFFFFu)), fabsf(half_to_f32<BF16>(u.x >> 16))),
+                                     fmaxf(fabsf(half_to_f32<BF16>(u.y & 0xFFFFu)), fabsf(half_to_f32<BF16>(u.y >> 16)))));
+            }
+            big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+            big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+            int e = int(__float_as_uint(big) >> 23) - 127 - 7;   // big in [2^(e + 7), 2^(e + 8))
+            if (!(big < INFINITY) || big < 1e-30f) e = 0;
+            const float down = __uint_as_float(uint32_t(127 - e) << 23);
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+              const uint2 u = *reinterpret_cast<const uint2 *>(qrow + j * 32 + col4 * 8);
+              qf[j][n][0] = pack_half2<false>(half_to_f32<BF16>(u.x & 0xFFFFu) * down, half_to_f32<BF16>(u.x >> 16) * down);
+              qf[j][n][1] = pack_half2<false>(half_to_f32<BF16>(u.y & 0xFFFFu) * down, half_to_f32<BF16>(u.y >> 16) * down);
+            }
+            mul *= __uint_as_float(uint32_t(127 + e) << 23);
+            if (c.key_scale) mul *= c.key_scale[comp.unit / p.sets];
+          } else {
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+              qf[j][n][0] = *reinterpret_cast<const uint32_t *>(qrow + j * 32 + col4 * 4);
+              qf[j][n][1] = *reinterpret_cast<const uint32_t *>(qrow + j * 32 + col4 * 4 + 16);
+            }
+          }
+          // this thread's results belong to columns 2 col4 and 2 col4 + 1
+          factor[n][0] = __shfl_sync(0xFFFFFFFFu, mul, col4 * 8);
+          factor[n][1] = __shfl_sync(0xFFFFFFFFu, mul, col4 * 8 + 4);
+          m[n][0] = m[n][1] = -INFINITY;
+          l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+          for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[j][n][i] = 0.f;
+        }
+        fresh = false;
+      }
+
+      const uint32_t ks = smem_u32(mine + stage * S::kSlot), vs = ks + S::kTokens * S::kRow;
+      // ---- S^T = K Q^T
+      float sc[kSubs][NT][4];
+#pragma unroll
+      for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[u][n][i] = 0.f;
+#pragma unroll
+      for (int u = 0; u < kSubs; ++u) {
+        if constexpr (F8) {
+#pragma unroll
+          for (int j = 0; j < kSteps; j += 2) {
+            if (j * 16 < dim) {
+              uint32_t r[4];   // tokens 0-7 and 8-15 of chunk j, then of chunk j + 1
+              ldmatrix_x4(r, ks + chunk_at<S::kChunks>(u * 16 + (lane & 15), j + (lane >> 4)));
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                if ((j + h) * 16 >= dim) break;   // an odd number of chunks: nobody has filled the last one
+                const uint32_t a[4] = {e4m3x2_to_f16x2(r[2 * h] & 0xFFFFu), e4m3x2_to_f16x2(r[2 * h + 1] & 0xFFFFu), e4m3x2_to_f16x2(r[2 * h] >> 16),
+                                       e4m3x2_to_f16x2(r[2 * h + 1] >> 16)};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma_16816<kMmaBf16>(sc[u][n], a, qf[j + h][n][0], qf[j + h][n][1]);
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kSteps; ++j) {
+            if (j * 16 < dim) {
+              uint32_t a[4];
+              ldmatrix_x4(a, ks + chunk_at<S::kChunks>(u * 16 + (lane & 15), 2 * j + (lane >> 4)));
+              if (j * 16 + 8 >= dim) a[2] = a[3] = 0u;   // half a step: nobody has filled the other half
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma_16816<kMmaBf16>(sc[u][n], a, qf[j][n][0], qf[j][n][1]);
+            }
+          }
+        }
+      }
+      // ---- softmax
+      const int pos0 = comp.first + comp.tile * S::kTile + warp * S::kTokens;
+      bool grow = false;
+      float top[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[u][n][i] *= factor[n][i & 1];
+      if (pos0 + S::kTokens > comp.end) {
+#pragma unroll
+        for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (pos0 + u * 16 + row8 + 8 * (i >> 1) >= comp.end) sc[u][n][i] = -INFINITY;
+      }
+#pragma unroll
+      for (int u = 0; u < kSubs; ++u)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top[n][i & 1] = fmaxf(top[n][i & 1], sc[u][n][i]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) grow = grow || top[n][0] > m[n][0] + (kLazy + kBelow) || top[n][1] > m[n][1] + (kLazy + kBelow);
+      if (__any_sync(0xFFFFFFFFu, grow)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float t = top[n][h];
+#pragma unroll
+            for (int i = 4; i < 32; i <<= 1) t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, i));
+            t = fmaxf(t - kBelow, m[n][h]);
+            const float alpha = ex2(m[n][h] - finite_ref(t));
+            m[n][h] = t;
+            l[n][h] *= alpha;
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+              acc[j][n][h] *= alpha;
+              acc[j][n][2 + h] *= alpha;
+            }
+          }
+      }
+      // ---- P, its sum, and O^T += V^T P^T
+#pragma unroll
+      for (int u = 0; u < kSubs; ++u) {
+        uint32_t pt[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float r0 = finite_ref(m[n][0]), r1 = finite_ref(m[n][1]);
+          const float w[4] = {ex2(sc[u][n][0] - r0), ex2(sc[u][n][1] - r1), ex2(sc[u][n][2] - r0), ex2(sc[u][n][3] - r1)};
+          l[n][0] += w[0] + w[2];
+          l[n][1] += w[1] + w[3];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) pt[n][h] = movmatrix_trans(pack_half2<kMmaBf16>(w[2 * h], w[2 * h + 1]));
+        }
+        const int tok = u * 16 + (lane & 7) + 8 * (lane >> 4), half8 = (lane >> 3) & 1;
+        if constexpr (F8) {
+          // chunk j holds head_dim 16 j ..: rows 2 i and 2 i + 1 of the result come from the low and the high byte of its pair i
+#pragma unroll
+          for (int j = 0; j < kSteps; j += 2) {
+            if (j * 16 < dim) {
+              uint32_t r[4];   // chunk j, tokens 0-7; chunk j + 1, tokens 0-7; chunk j, tokens 8-15; chunk j + 1, tokens 8-15
+              ldmatrix_x4_trans(r, vs + chunk_at<S::kChunks>(tok, j + half8));
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                if ((j + h) * 16 >= dim) break;
+                const uint32_t t0 = __byte_perm(r[h], 0, 0x3120), t1 = __byte_perm(r[h + 2], 0, 0x3120);
+                const uint32_t a[4] = {e4m3x2_to_f16x2(t0 & 0xFFFFu), e4m3x2_to_f16x2(t0 >> 16), e4m3x2_to_f16x2(t1 & 0xFFFFu), e4m3x2_to_f16x2(t1 >> 16)};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma_16816<kMmaBf16>(acc[j + h][n], a, pt[n][0], pt[n][1]);
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kSteps; ++j) {
+            if (j * 16 < dim) {
+              uint32_t a[4];
+              ldmatrix_x4_trans(a, vs + chunk_at<S::kChunks>(tok, 2 * j + half8));
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma_16816<kMmaBf16>(acc[j][n], a, pt[n][0], pt[n][1]);
+            }
+          }
+        }
+      }
+
+      const bool unit_ends = comp.tile + 1 == comp.tiles;
+      if (unit_ends || x + 1 == count) {
+        // ---- the four warps' parts meet in shared memory, each in the slot whose tokens it has just used
+        __syncwarp();
+        float *own = reinterpret_cast<float *>(mine + stage * S::kSlot);   // [DP][cols]
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int j = 0; j < kSteps; ++j) {
+            const int d0 = F8 ? j * 16 + 2 * row8 : j * 16 + row8, d1 = F8 ? d0 + 1 : d0 + 8;
+            *reinterpret_cast<float2 *>(own + d0 * S::kCols + n * 8 + 2 * col4) = make_float2(acc[j][n][0], acc[j][n][1]);
+            *reinterpret_cast<float2 *>(own + d1 * S::kCols + n * 8 + 2 * col4) = make_float2(acc[j][n][2], acc[j][n][3]);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 4; i < 32; i <<= 1) l[n][h] += __shfl_xor_sync(0xFFFFFFFFu, l[n][h], i);
+            if (lane < 4) {
+              stat_m[warp][n * 8 + 2 * col4 + h] = m[n][h];
+              stat_l[warp][n * 8 + 2 * col4 + h] = l[n][h];
+            }
+          }
+        }
+        __syncthreads();
+        const int kv = comp.unit / p.sets, set = comp.unit - kv * p.sets;
+        const int cols = min(S::kCols, p.group - set * S::kCols);
+        const bool begins = segment > 0 || first_tile == 0;   // not the unit that the block before began
+        const bool whole = begins && unit_ends;
+        float *out_part = p.parts + (2 * int64_t(blockIdx.x) + (begins ? 1 : 0)) * part_floats(S::kCols, dim);
+        const float vscale = F8 && c.value_scale ? c.value_scale[kv] : 1.f;
+        for (int i = threadIdx.x; i < NT * dim; i += kThreads) {
+          const int n = i / dim, d = i - n * dim;
+          float sum[8] = {};
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float4 *src = reinterpret_cast<const float4 *>(smem + (w * kStages + stage) * S::kSlot) + (d * S::kCols + n * 8) / 4;
+            const float4 a = src[0], b = src[1];
+            const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int h = 0; h < 8; ++h) {
+              float top_m = stat_m[0][n * 8 + h];
+#pragma unroll
+              for (int w2 = 1; w2 < kWarps; ++w2) top_m = fmaxf(top_m, stat_m[w2][n * 8 + h]);
+              sum[h] = fmaf(v[h], ex2(stat_m[w][n * 8 + h] - finite_ref(top_m)), sum[h]);
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 8; ++h) {
+            const int col = n * 8 + h;
+            if (col >= cols) break;
+            float top_m = stat_m[0][col], sum_l = 0.f;
+#pragma unroll
+            for (int w2 = 1; w2 < kWarps; ++w2) top_m = fmaxf(top_m, stat_m[w2][col]);
+#pragma unroll
+            for (int w2 = 0; w2 < kWarps; ++w2) sum_l = fmaf(stat_l[w2][col], ex2(stat_m[w2][col] - finite_ref(top_m)), sum_l);
+            const int head = kv * p.group + set * S::kCols + col;
+            if (whole) {
+              p.out[comp.seq * p.o_seq + head * p.o_head + d] = f32_to_half<BF16>(sum[h] / sum_l * vscale);
+              if (d == 0 && p.lse) p.lse[int64_t(comp.seq) * p.heads + head] = (finite_ref(top_m) + log2f(sum_l)) * 0.6931471805599453f;
+            } else {
+              out_part[int64_t(col) * dim + d] = sum[h];
+              if (d == 0) {
+                out_part[int64_t(S::kCols) * dim + 2 * col] = top_m;
+                out_part[int64_t(S::kCols) * dim + 2 * col + 1] = sum_l;
+              }
+            }
+          }
+        }
+        __syncthreads();   // before the slots are filled again
+        fresh = true;
+        ++segment;
+      }
+      __syncwarp();
+      if (x + kStages < count) issue(stage);
+      cp_async_commit();
+      if (++stage == kStages) stage = 0;
+      if (x + 1 < count) advance<S::kTile>(p, units, comp);
+    }
+    cp_async_wait<0>();
+  }
+
+  // ---- sequences of which nothing is seen
+  for (int s = blockIdx.x; s < c.table.sequences; s += gridDim.x) {
+    const Seen see = seen_of(c.table, p.lengths[s], p.window);
+    if (see.cut && threadIdx.x == 0) atomicExch(c.error, int(ERR_BAD_PAGE));
+    if (see.end > see.first) continue;
+    for (int i = threadIdx.x; i < p.heads * dim; i += kThreads) {
+      const int h = i / dim;
+      p.out[s * p.o_seq + h * p.o_head + (i - h * dim)] = 0;
+    }
+    if (p.lse)
+      for (int h = threadIdx.x; h < p.heads; h += kThreads) p.lse[int64_t(s) * p.heads + h] = -INFINITY;
   }
 }
 
-// One block per sequence and query head; a warp per token, eight elements of head_dim to a lane.
-template <bool BF16, bool F8>
-__global__ void __launch_bounds__(kWarps * 32) paged_attention_kernel(const __grid_constant__ PagedAttParams p) {
-  __shared__ float sm[kWarps], sl[kWarps], so[kWarps][256];
+// Block (i - 1, y): the unit that border i cuts first, columns y, y + gridDim.y, ...
+template <bool BF16, bool F8, int DP, int NT>
+__global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_constant__ PagedAttParams p) {
+  using S = Shape<F8, DP, NT>;
+  __shared__ int64_t pre[kThreads + 1];
+  __shared__ Place found;
   const PagedCache &c = p.c;
-  const int s = blockIdx.y, h = blockIdx.x, kvh = h / p.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Seen see = seen_of(c.table, p.lengths[s], p.window);
-  const int first = see.first, len = see.end;
-  if (see.cut && threadIdx.x == 0) atomicExch(c.error, int(ERR_BAD_PAGE));
-  const float ks = F8 && c.key_scale ? c.key_scale[kvh] : 1.f, vs = F8 && c.value_scale ? c.value_scale[kvh] : 1.f;
-  const int d0 = lane * 8;
-  const bool mine = d0 < c.dim;
-  const int size = F8 ? 1 : 2;
-  float q[8], o[8] = {}, m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) q[i] = mine ? half_to_f32<BF16>(p.q[s * p.q_seq + h * p.q_head + d0 + i]) * p.scale * ks : 0.f;
-  for (int t = first + warp; t < len; t += kWarps) {
-    const int page = page_of(c.table, s, t), slot = t % c.table.page_size;
-    const bool held = page >= 0;
-    if (!held && lane == 0) atomicExch(c.error, int(ERR_BAD_PAGE));
-    float k[8] = {}, v[8] = {};
-    if (held && mine) {
-      load8<BF16, F8>(c.keys + page * c.key_page + kvh * c.key_head + slot * c.key_token + d0 * size, k);
-      load8<BF16, F8>(c.values + page * c.value_page + kvh * c.value_head + slot * c.value_token + d0 * size, v);
+  const int units = c.kv_heads * p.sets, dim = c.dim;
+  const int64_t i = int64_t(blockIdx.x) + 1;
+  // The lengths may be read before the wait: the kernel ahead let this one start behind its own wait for everything before it.
+  const int64_t total = count_tiles<S::kTile>(p, units, pre), per = share_of(total, p.blocks, p.least);
+  bool cut = i * per < total;
+  Place at{};
+  int64_t begin = 0, end = 0;
+  int unit = 0;
+  if (cut) {
+    at = locate<S::kTile>(p, units, pre, i * per, &found);
+    const int tiles = tiles_of(seen_of(c.table, p.lengths[at.seq], p.window), S::kTile);
+    unit = min(units - 1, int(at.rest / max(1, tiles)));
+    begin = i * per - (at.rest - int64_t(unit) * tiles);
+    end = begin + tiles;
+    cut = first_cut(i, per, begin, end);
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  if (!cut) return;
+  const int kv = unit / p.sets, set = unit - kv * p.sets, cols = min(S::kCols, p.group - set * S::kCols);
+  const int64_t b0 = begin / per, b1 = (end - 1) / per, floats = part_floats(S::kCols, dim);
+  const float vscale = F8 && c.value_scale ? c.value_scale[kv] : 1.f;
+  for (int col = blockIdx.y; col < cols; col += gridDim.y) {
+    float m = -INFINITY;
+    for (int64_t b = b0; b <= b1; ++b) m = fmaxf(m, p.parts[part_slot(b, per, begin) * floats + int64_t(S::kCols) * dim + 2 * col]);
+    const float ref = finite_ref(m);
+    const int head = kv * p.group + set * S::kCols + col;
+    for (int d = threadIdx.x; d < dim; d += kThreads) {
+      float l = 0.f, sum = 0.f;
+      for (int64_t b = b0; b <= b1; ++b) {
+        const float *part = p.parts + part_slot(b, per, begin) * floats;
+        const float w = ex2(part[int64_t(S::kCols) * dim + 2 * col] - ref);
+        l = fmaf(part[int64_t(S::kCols) * dim + 2 * col + 1], w, l);
+        sum = fmaf(part[int64_t(col) * dim + d], w, sum);
+      }
+      p.out[at.seq * p.o_seq + head * p.o_head + d] = f32_to_half<BF16>(sum / l * vscale);
+      if (d == 0 && p.lse) p.lse[int64_t(at.seq) * p.heads + head] = (ref + log2f(l)) * 0.6931471805599453f;
     }
-    float dot = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) dot = fmaf(q[i], k[i], dot);
-#pragma unroll
-    for (int i = 16; i > 0; i >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, i);
-    const float mn = fmaxf(m, dot), base = mn == -INFINITY ? 0.f : mn;
-    const float alpha = __expf(m - base), w = __expf(dot - base);
-    m = mn;
-    l = l * alpha + w;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = fmaf(w, v[i], o[i] * alpha);
   }
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) so[warp][d0 + i] = o[i];
-  __syncthreads();
-  float mx = -INFINITY, total = 0.f;
-  for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm[w]);
-  const float base = mx == -INFINITY ? 0.f : mx;
-  for (int w = 0; w < kWarps; ++w) total += sl[w] * __expf(sm[w] - base);
-  for (int d = threadIdx.x; d < c.dim; d += kWarps * 32) {
-    float sum = 0.f;
-    for (int w = 0; w < kWarps; ++w) sum += so[w][d] * __expf(sm[w] - base);
-    p.out[s * p.o_seq + h * p.o_head + d] = f32_to_half<BF16>(len > first ? sum / total * vs : 0.f);
-  }
-  if (p.lse && threadIdx.x == 0) p.lse[int64_t(s) * p.heads + h] = base + logf(total);
 }
 
 void require(bool ok, const char *what) {
   if (!ok) throw std::invalid_argument(what);
+}
+
+// Columns of a product: 16 for more than eight heads to a KV head, where the registers allow it.
+int columns(int64_t group, int64_t dim) { return group > 8 && dim <= 128 ? 16 : 8; }
+
+template <typename... KArgs, typename... Args>
+void launch_dependent(void (*kernel)(KArgs...), dim3 grid, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  GCB_CUDA(cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...));
+  count_launch();
+}
+
+template <bool BF16, bool F8, int DP, int NT> void launch(PagedAttParams p, DeviceState &dev, cudaStream_t stream) {
+  using S = Shape<F8, DP, NT>;
+  auto kernel = paged_attention_kernel<BF16, F8, DP, NT>;
+  static int resident[64] = {};   // blocks of an SM
+  int &r = resident[dev.device & 63];
+  if (!r) {
+    int n = 0;
+    GCB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
+    GCB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, S::kBytes));
+    r = std::max(1, n);
+  }
+  p.blocks = std::min(kMaxBlocks, dev.sm_count * r);
+  p.least = 1;
+  launch_dependent(kernel, dim3(unsigned(p.blocks)), S::kBytes, stream, p);
+  if (p.blocks > 1) launch_dependent(paged_join_kernel<BF16, F8, DP, NT>, dim3(unsigned(p.blocks - 1), 4), 0, stream, p);
+}
+
+template <bool BF16, bool F8> void launch(const PagedAttParams &p, int cols, DeviceState &dev, cudaStream_t stream) {
+  const int dim = p.c.dim;
+  if (dim <= 64) cols == 16 ? launch<BF16, F8, 64, 2>(p, dev, stream) : launch<BF16, F8, 64, 1>(p, dev, stream);
+  else if (dim <= 128) cols == 16 ? launch<BF16, F8, 128, 2>(p, dev, stream) : launch<BF16, F8, 128, 1>(p, dev, stream);
+  else launch<BF16, F8, 256, 1>(p, dev, stream);
 }
 
 } // namespace
@@ -115,7 +630,7 @@ void require(bool ok, const char *what) {
 size_t paged_attention_workspace(int64_t heads, int64_t kv_heads, int64_t head_dim) {
   require(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads < 65536, "paged attention: heads must be a multiple of kv_heads");
   require(head_dim > 0 && head_dim <= 256, "paged attention: head_dim must be at most 256");
-  return 16;
+  return size_t(2) * kMaxBlocks * size_t(part_floats(columns(heads / kv_heads, head_dim), int(head_dim))) * sizeof(float);
 }
 
 void paged_attention(const gcb200_paged_cache &cache, const PagedAttentionArgs &a, cudaStream_t stream) {
@@ -125,28 +640,28 @@ void paged_attention(const gcb200_paged_cache &cache, const PagedAttentionArgs &
   require((reinterpret_cast<uintptr_t>(a.workspace) & 15) == 0, "paged attention: the workspace must be 16-byte aligned");
   require(a.workspace_bytes >= paged_attention_workspace(a.heads, cache.kv_heads, cache.head_dim), "paged attention: the workspace is too small");
   require(a.window >= 0, "paged attention: negative window");
-  require(cache.sequences < 65536, "paged attention: more than 65535 sequences");
   if (cache.sequences == 0) return;
   DeviceState &dev = device_state();
   p.c.error = dev.d_error;
   p.q = static_cast<const uint16_t *>(a.q);
   p.out = static_cast<uint16_t *>(a.out);
-  p.q_seq = a.q_stride[0];
-  p.q_head = a.q_stride[1];
-  p.o_seq = a.out_stride[0];
-  p.o_head = a.out_stride[1];
+  p.q_seq = cache.sequences > 1 ? a.q_stride[0] : 0;
+  p.q_head = a.heads > 1 ? a.q_stride[1] : 0;
+  p.o_seq = cache.sequences > 1 ? a.out_stride[0] : 0;
+  p.o_head = a.heads > 1 ? a.out_stride[1] : 0;
+  p.q_aligned = ((reinterpret_cast<uintptr_t>(a.q) | uintptr_t(2 * p.q_seq) | uintptr_t(2 * p.q_head)) & 15) == 0;
+  p.same_strides = p.c.key_page == p.c.value_page && p.c.key_token == p.c.value_token;
   p.lengths = a.lengths;
   p.lse = a.lse;
-  p.scale = a.scale;
+  p.parts = static_cast<float *>(a.workspace);
+  p.scale_log2e = a.scale * 1.4426950408889634f;
   p.heads = int(a.heads);
   p.group = int(a.heads / cache.kv_heads);
+  const int cols = columns(p.group, cache.head_dim);
+  p.sets = (p.group + cols - 1) / cols;
   p.window = int(std::min<int64_t>(a.window, INT32_MAX));
-  const dim3 grid(unsigned(a.heads), unsigned(cache.sequences));
   const bool bf16 = cache.dtype == GCB200_BF16, f8 = cache.cache_dtype == GCB200_F8_E4M3;
-  (bf16 ? (f8 ? paged_attention_kernel<true, true> : paged_attention_kernel<true, false>)
-        : (f8 ? paged_attention_kernel<false, true> : paged_attention_kernel<false, false>))<<<grid, kWarps * 32, 0, stream>>>(p);
-  GCB_CUDA(cudaGetLastError());
-  count_launch();
+  (bf16 ? (f8 ? launch<true, true> : launch<true, false>) : (f8 ? launch<false, true> : launch<false, false>))(p, cols, dev, stream);
 }
 
 } // namespace gcb

@@ -41,4 +41,20 @@ GCB_HD Seen seen_of(const PageTable &t, int length, int window) {
   return s;
 }
 
+// How the tokens that all queries see are shared out among `blocks` thread blocks.  A unit is what one set of query heads of one
+// KV head does for one sequence; its tokens are cut into tiles, and the tiles of all units, sequence by sequence and unit by unit
+// inside, are one row of `total` that is cut into equal parts: block i takes [i per, (i + 1) per).  A unit may be cut by the borders
+// of several blocks; each then keeps a part of its softmax, and the parts are joined in the order of the blocks.
+GCB_HD int tiles_of(const Seen &s, int tile) { return (s.end - s.first + tile - 1) / tile; }
+GCB_HD int64_t share_of(int64_t total, int blocks, int least) {
+  const int64_t per = (total + blocks - 1) / blocks;
+  return per < least ? least : per;
+}
+// A block keeps at most two parts: of the unit that it continues (0) and of one that it begins and does not end (1).
+GCB_HD int64_t part_slot(int64_t block, int64_t per, int64_t unit_begin) { return 2 * block + (unit_begin >= block * per ? 1 : 0); }
+// Whether border number `i` (the tile i per) is the first one inside the unit [begin, end): the join of its parts belongs to it.
+GCB_HD bool first_cut(int64_t i, int64_t per, int64_t begin, int64_t end) {
+  return begin < i * per && i * per < end && begin >= (i - 1) * per;
+}
+
 } // namespace gcb

@@ -118,6 +118,10 @@ extern "C" void t_seen_of(int max_pages, int page_size, int length, int window, 
   gcb::Seen s = gcb::seen_of(t, length, window);
   out[0] = s.first; out[1] = s.end; out[2] = s.cut;
 }
+extern "C" int64_t t_share_of(int64_t total, int blocks, int least) { return gcb::share_of(total, blocks, least); }
+extern "C" int64_t t_part_slot(int64_t block, int64_t per, int64_t begin) { return gcb::part_slot(block, per, begin); }
+extern "C" int t_first_cut(int64_t i, int64_t per, int64_t begin, int64_t end) { return gcb::first_cut(i, per, begin, end); }
+extern "C" int t_tiles_of(int first, int end, int tile) { return gcb::tiles_of(gcb::Seen{first, end, false}, tile); }
 """
 
 
@@ -130,6 +134,9 @@ def index(tmp_path_factory):
     l = C.CDLL(str(so))
     l.t_page_of.argtypes = [C.c_void_p, C.c_int64] + [C.c_int] * 6
     l.t_seen_of.argtypes = [C.c_int] * 4 + [C.c_void_p]
+    for name, args in (("t_share_of", [C.c_int64, C.c_int, C.c_int]), ("t_part_slot", [C.c_int64] * 3), ("t_first_cut", [C.c_int64] * 4)):
+        getattr(l, name).argtypes = args
+    l.t_share_of.restype = l.t_part_slot.restype = C.c_int64
     return l
 
 
@@ -157,3 +164,44 @@ def test_seen_positions(index):
     assert seen(7, 0) == (0, 7, 0) and seen(7, 7) == (0, 7, 0) and seen(7, 8) == (0, 7, 0) and seen(7, 2) == (5, 7, 0)
     assert seen(24, 0) == (0, 24, 0) and seen(25, 0) == (0, 24, 1) and seen(2147483647, 1) == (23, 24, 1)
     assert seen(3, 0, max_pages=0) == (0, 0, 1)
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_every_tile_has_one_block_and_every_cut_unit_one_join(index, seed):
+    """The blocks' shares, walked as the kernel walks them: each tile once, no more than two parts to a block, and the parts that
+    the join of a cut unit reads are those that were written for it."""
+    r = np.random.RandomState(seed)
+    tile, units, blocks, least = int(r.choice([64, 128])), int(r.choice([1, 2, 8, 40])), int(r.choice([1, 2, 7, 148, 592])), int(r.choice([1, 1, 2, 5]))
+    lengths = [int(x) for x in r.randint(0, r.choice([2, 100, 3000]), r.choice([1, 3, 50]))]
+    begins, at = [], 0
+    for n in lengths:
+        k = index.t_tiles_of(0, n, tile)
+        assert k == -(-n // tile)
+        begins += [(at + u * k, at + (u + 1) * k) for u in range(units) if k]
+        at += k * units
+    total, per = at, index.t_share_of(at, blocks, least)
+    assert per >= least and per * blocks >= total
+    written, whole = {}, set()
+    for b in range(blocks):
+        lo, hi = b * per, min(total, (b + 1) * per)
+        for u, (x, y) in enumerate(begins):
+            if max(lo, x) < min(hi, y):
+                if lo <= x and y <= hi:
+                    whole.add(u)
+                else:
+                    slot = 2 * b + (1 if x >= lo else 0)
+                    assert slot not in written and slot < 2 * blocks
+                    written[slot] = u
+    joined = set()
+    for i in range(1, blocks):
+        if i * per >= total:
+            continue
+        u = next(k for k, (x, y) in enumerate(begins) if x <= i * per < y)
+        x, y = begins[u]
+        if index.t_first_cut(i, per, x, y):
+            assert u not in joined
+            joined.add(u)
+            slots = [index.t_part_slot(b, per, x) for b in range(x // per, (y - 1) // per + 1)]
+            assert len(slots) > 1 and all(written[s] == u for s in slots)
+            assert slots == [s for s in sorted(written) if written[s] == u]
+    assert joined == set(written.values()) and not joined & whole and len(joined) + len(whole) == len(begins)
