@@ -237,7 +237,7 @@ PagedCache checked_cache(const gcb200_paged_cache &c, bool writes) {
   require(c.keys && c.values && (c.page_table || c.sequences == 0 || c.max_pages == 0), "paged cache: null pointer");
   require(c.pages > 0 && c.page_size > 0 && c.kv_heads > 0 && c.sequences >= 0 && c.max_pages >= 0, "paged cache: sizes must be positive");
   require(c.pages < (int64_t(1) << 31) && c.sequences < (int64_t(1) << 31) && c.kv_heads < 65536 && c.page_size <= (int64_t(1) << 30) &&
-              c.max_pages < (int64_t(1) << 31) && c.page_size * c.max_pages < (int64_t(1) << 31),
+              c.max_pages < (int64_t(1) << 31) && c.page_size * c.max_pages <= (int64_t(1) << 31) - 65536,
           "paged cache: positions and page numbers are 32-bit");
   const int size = c.cache_dtype == GCB200_F8_E4M3 ? 1 : 2;
   require(c.head_dim >= 8 && c.head_dim <= kMaxDim && c.head_dim * size % 16 == 0,

@@ -153,7 +153,8 @@ template <int CHUNKS> __device__ __forceinline__ uint32_t chunk_at(int r, int ch
   else return uint32_t(r * CHUNKS + (ch ^ ((r >> 1) & 3))) * 16u;
 }
 
-template <bool BF16, bool F8, int DP, int NT>
+// FULL: head_dim is DP, and nothing has to ask where it ends.
+template <bool BF16, bool F8, int DP, int NT, bool FULL>
 __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_constant__ PagedAttParams p) {
   using S = Shape<F8, DP, NT>;
   constexpr bool kMmaBf16 = BF16 && !F8;
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
 
   const PagedCache &c = p.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row8 = lane >> 2, col4 = lane & 3;
-  const int units = c.kv_heads * p.sets, dim = c.dim;
+  const int units = c.kv_heads * p.sets, dim = FULL ? DP : c.dim;
   pdl_wait();
   pdl_launch_dependents();   // behind the wait: what starts now finds everything before this kernel done
 
@@ -186,34 +187,56 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
 
     uint8_t *mine = smem + warp * kStages * S::kSlot;
     uint8_t *qring = smem + kWarps * kStages * S::kSlot;
-    // ---- what the next tile to fetch needs: this lane's token's page and slot
-    int next_page = -1, next_slot = 0, next_seq = 0, next_unit = 0, fetched = 0, segments = 0;
-    bool next_new = true;
+    // ---- what the next tile to fetch needs: this lane's token's entry of the page table, and its place in the page
+    int next_page = -1, next_slot = 0, fetched = 0, segments = 0;
+    int entry = 0, slot = 0;              // of this lane's token of tile `ahead`
+    int ahead_kv = 0, ahead_set = 0, next_kv = 0, next_set = 0, next_seq = 0;
+    bool next_new = true, opened = true;
+    const int step_entry = S::kTile / c.table.page_size, step_slot = S::kTile % c.table.page_size;
     auto look_up = [&]() {
-      next_seq = ahead.seq;
-      next_unit = ahead.unit;
-      next_new = fetched == 0 || ahead.tile == 0;
+      if (fetched >= count) return;
       const int pos = ahead.first + ahead.tile * S::kTile + warp * S::kTokens + lane;
+      if (opened) {   // divisions once per unit; from tile to tile the place moves by the same step
+        entry = pos / c.table.page_size;
+        slot = pos - entry * c.table.page_size;
+        ahead_kv = ahead.unit / p.sets;
+        ahead_set = ahead.unit - ahead_kv * p.sets;
+      }
+      next_new = opened;
+      next_seq = ahead.seq;
+      next_kv = ahead_kv;
+      next_set = ahead_set;
+      next_slot = slot;
       next_page = -1;
-      next_slot = 0;
       if (lane < S::kTokens && pos < ahead.end) {
-        next_page = page_of(c.table, ahead.seq, pos);
-        next_slot = pos % c.table.page_size;
+        next_page = page_at(c.table, ahead.seq, entry);
         if (next_page < 0) atomicExch(c.error, int(ERR_BAD_PAGE));
       }
-      if (++fetched < count) advance<S::kTile>(p, units, ahead);
+      entry += step_entry;
+      slot += step_slot;
+      if (slot >= c.table.page_size) {
+        slot -= c.table.page_size;
+        ++entry;
+      }
+      opened = false;
+      if (++fetched < count) {
+        advance<S::kTile>(p, units, ahead);
+        opened = ahead.tile == 0;
+      }
     };
-    const int lane_row = lane / S::kChunks, lane_chunk = lane % S::kChunks;
-    const bool lane_copies = lane_chunk * 16 < dim * (F8 ? 1 : 2);
+    // Copies: eight lanes (four for rows of 64 bytes) take one row's chunks, and go on every 128 bytes and every kRows rows.
+    constexpr int kLanes = S::kChunks < 8 ? S::kChunks : 8, kRows = 32 / kLanes, kPieces = S::kChunks / kLanes;
+    const int lane_row = lane / kLanes, lane_chunk = lane % kLanes;
+    const uint32_t copy_even = chunk_at<S::kChunks>(lane_row, lane_chunk), copy_odd = chunk_at<S::kChunks>(lane_row + kRows, lane_chunk) - kRows * S::kRow;
+    const uint32_t mine_s = smem_u32(mine);
     auto issue = [&](int stage) {
-      const int kv = next_unit / p.sets, set = next_unit - kv * p.sets;
       if (next_new) {
         uint8_t *dst = qring + (segments % (kStages + 1)) * S::kQ;
         ++segments;
         for (int i = threadIdx.x; i < S::kCols * (DP / 8); i += kThreads) {
-          const int col = i / (DP / 8), d = (i - col * (DP / 8)) * 8, in_group = set * S::kCols + col;
+          const int col = i / (DP / 8), d = (i - col * (DP / 8)) * 8, in_group = next_set * S::kCols + col;
           const bool there = in_group < p.group && d < dim;
-          const uint16_t *src = p.q + (there ? next_seq * p.q_seq + (kv * p.group + in_group) * p.q_head + d : 0);
+          const uint16_t *src = p.q + (there ? next_seq * p.q_seq + (next_kv * p.group + in_group) * p.q_head + d : 0);
           uint8_t *to = dst + col * S::kQRow + d * 2;
           if (p.q_aligned) {
             cp_async_16(smem_u32(to), src, there ? 16u : 0u);
@@ -225,17 +248,21 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
       }
       const int64_t koff = next_page < 0 ? -1 : next_page * c.key_page + next_slot * c.key_token;
       const int64_t voff = p.same_strides || next_page < 0 ? koff : next_page * c.value_page + next_slot * c.value_token;
-      const uint8_t *kbase = c.keys + kv * c.key_head + lane_chunk * 16, *vbase = c.values + kv * c.value_head + lane_chunk * 16;
-      const uint32_t dst = smem_u32(mine + stage * S::kSlot);
+      const uint8_t *kbase = c.keys + next_kv * c.key_head + lane_chunk * 16, *vbase = c.values + next_kv * c.value_head + lane_chunk * 16;
+      const uint32_t even = mine_s + stage * S::kSlot + copy_even, odd = mine_s + stage * S::kSlot + copy_odd;
 #pragma unroll
-      for (int i = 0; i < S::kTokens * S::kChunks / 32; ++i) {
-        const int r = i * (32 / S::kChunks) + lane_row;
-        const int64_t ko = __shfl_sync(0xFFFFFFFFu, koff, r);
-        const int64_t vo = p.same_strides ? ko : __shfl_sync(0xFFFFFFFFu, voff, r);
-        if (lane_copies) {
-          const uint32_t to = dst + chunk_at<S::kChunks>(r, lane_chunk), bytes = ko < 0 ? 0u : 16u;
-          cp_async_16(to, kbase + (ko < 0 ? 0 : ko), bytes);
-          cp_async_16(to + S::kTokens * S::kRow, vbase + (ko < 0 ? 0 : vo), bytes);
+      for (int i = 0; i < S::kTokens / kRows; ++i) {
+        const int64_t ko = __shfl_sync(0xFFFFFFFFu, koff, i * kRows + lane_row);
+        int64_t vo = ko;
+        if (!p.same_strides) vo = __shfl_sync(0xFFFFFFFFu, voff, i * kRows + lane_row);
+        const uint32_t bytes = ko < 0 ? 0u : 16u, to = (i & 1 ? odd : even) + i * kRows * S::kRow;
+        const uint8_t *kp = ko < 0 ? kbase : kbase + ko, *vp = ko < 0 ? vbase : vbase + vo;
+#pragma unroll
+        for (int e = 0; e < kPieces; ++e) {
+          if (FULL || (lane_chunk + e * kLanes) * 16 < dim * (F8 ? 1 : 2)) {
+            cp_async_16(to + e * 128, kp + e * 128, bytes);
+            cp_async_16(to + e * 128 + S::kTokens * S::kRow, vp + e * 128, bytes);
+          }
         }
       }
       look_up();
@@ -247,8 +274,20 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
       cp_async_commit();
     }
 
+    // Where this lane points the matrix loads of step j: four places, the rest is a constant distance (two with rows of 64 bytes).
+    const int k_row = lane & 15, k_chunk = lane >> 4, v_row = (lane & 7) + 8 * (lane >> 4), v_chunk = (lane >> 3) & 1;
+    uint32_t k_at[4], v_at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      k_at[i] = chunk_at<S::kChunks>(k_row, (2 * i + k_chunk) % S::kChunks);
+      v_at[i] = chunk_at<S::kChunks>(v_row, (2 * i + v_chunk) % S::kChunks);
+    }
+    // chunk pair `pair` (two chunks) of sixteen rows from row 16 u
+    auto pair_at = [](const uint32_t (&at)[4], int u, int pair) {
+      return at[pair & 3] + uint32_t((pair >> 2) * 128 + u * 16 * S::kRow);
+    };
     uint32_t qf[kSteps][NT][2];
-    float acc[kSteps][NT][4], m[NT][2], l[NT][2], factor[NT][2];
+    float acc[kSteps][NT][4], m[NT][2], ref[NT][2], l[NT][2], factor[NT][2];
     int stage = 0, segment = 0;
     bool fresh = true;   // the tile is the first one of its unit here
     for (int x = 0; x < count; ++x) {
@@ -294,6 +333,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
           factor[n][0] = __shfl_sync(0xFFFFFFFFu, mul, col4 * 8);
           factor[n][1] = __shfl_sync(0xFFFFFFFFu, mul, col4 * 8 + 4);
           m[n][0] = m[n][1] = -INFINITY;
+          ref[n][0] = ref[n][1] = 0.f;
           l[n][0] = l[n][1] = 0.f;
 #pragma unroll
           for (int j = 0; j < kSteps; ++j)
@@ -303,42 +343,42 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
         fresh = false;
       }
 
-      const uint32_t ks = smem_u32(mine + stage * S::kSlot), vs = ks + S::kTokens * S::kRow;
+      const uint32_t ks = mine_s + stage * S::kSlot, vs = ks + S::kTokens * S::kRow;
       // ---- S^T = K Q^T
-      float sc[kSubs][NT][4];
+      float sc[kSubs][NT][4], sd[kSubs][NT][4];   // even and odd steps: one chain of dependent products half as long
 #pragma unroll
       for (int u = 0; u < kSubs; ++u)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[u][n][i] = 0.f;
+          for (int i = 0; i < 4; ++i) sc[u][n][i] = sd[u][n][i] = 0.f;
 #pragma unroll
       for (int u = 0; u < kSubs; ++u) {
         if constexpr (F8) {
 #pragma unroll
           for (int j = 0; j < kSteps; j += 2) {
-            if (j * 16 < dim) {
+            if (FULL || j * 16 < dim) {
               uint32_t r[4];   // tokens 0-7 and 8-15 of chunk j, then of chunk j + 1
-              ldmatrix_x4(r, ks + chunk_at<S::kChunks>(u * 16 + (lane & 15), j + (lane >> 4)));
+              ldmatrix_x4(r, ks + pair_at(k_at, u, j / 2));
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                if ((j + h) * 16 >= dim) break;   // an odd number of chunks: nobody has filled the last one
+                if (!FULL && (j + h) * 16 >= dim) break;   // an odd number of chunks: nobody has filled the last one
                 const uint32_t a[4] = {e4m3x2_to_f16x2(r[2 * h] & 0xFFFFu), e4m3x2_to_f16x2(r[2 * h + 1] & 0xFFFFu), e4m3x2_to_f16x2(r[2 * h] >> 16),
                                        e4m3x2_to_f16x2(r[2 * h + 1] >> 16)};
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma_16816<kMmaBf16>(sc[u][n], a, qf[j + h][n][0], qf[j + h][n][1]);
+                for (int n = 0; n < NT; ++n) mma_16816<kMmaBf16>(h ? sd[u][n] : sc[u][n], a, qf[j + h][n][0], qf[j + h][n][1]);
               }
             }
           }
         } else {
 #pragma unroll
           for (int j = 0; j < kSteps; ++j) {
-            if (j * 16 < dim) {
+            if (FULL || j * 16 < dim) {
               uint32_t a[4];
-              ldmatrix_x4(a, ks + chunk_at<S::kChunks>(u * 16 + (lane & 15), 2 * j + (lane >> 4)));
-              if (j * 16 + 8 >= dim) a[2] = a[3] = 0u;   // half a step: nobody has filled the other half
+              ldmatrix_x4(a, ks + pair_at(k_at, u, j));
+              if (!FULL && j * 16 + 8 >= dim) a[2] = a[3] = 0u;   // half a step: nobody has filled the other half
 #pragma unroll
-              for (int n = 0; n < NT; ++n) mma_16816<kMmaBf16>(sc[u][n], a, qf[j][n][0], qf[j][n][1]);
+              for (int n = 0; n < NT; ++n) mma_16816<kMmaBf16>(j & 1 ? sd[u][n] : sc[u][n], a, qf[j][n][0], qf[j][n][1]);
             }
           }
         }
@@ -354,7 +394,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[u][n][i] *= factor[n][i & 1];
+          for (int i = 0; i < 4; ++i) sc[u][n][i] = (sc[u][n][i] + sd[u][n][i]) * factor[n][i & 1];
       if (pos0 + S::kTokens > comp.end) {
 #pragma unroll
         for (int u = 0; u < kSubs; ++u)
@@ -381,7 +421,8 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
 #pragma unroll
             for (int i = 4; i < 32; i <<= 1) t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, i));
             t = fmaxf(t - kBelow, m[n][h]);
-            const float alpha = ex2(m[n][h] - finite_ref(t));
+            ref[n][h] = finite_ref(t);
+            const float alpha = ex2(m[n][h] - ref[n][h]);
             m[n][h] = t;
             l[n][h] *= alpha;
 #pragma unroll
@@ -397,24 +438,22 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
         uint32_t pt[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const float r0 = finite_ref(m[n][0]), r1 = finite_ref(m[n][1]);
-          const float w[4] = {ex2(sc[u][n][0] - r0), ex2(sc[u][n][1] - r1), ex2(sc[u][n][2] - r0), ex2(sc[u][n][3] - r1)};
+          const float w[4] = {ex2(sc[u][n][0] - ref[n][0]), ex2(sc[u][n][1] - ref[n][1]), ex2(sc[u][n][2] - ref[n][0]), ex2(sc[u][n][3] - ref[n][1])};
           l[n][0] += w[0] + w[2];
           l[n][1] += w[1] + w[3];
 #pragma unroll
           for (int h = 0; h < 2; ++h) pt[n][h] = movmatrix_trans(pack_half2<kMmaBf16>(w[2 * h], w[2 * h + 1]));
         }
-        const int tok = u * 16 + (lane & 7) + 8 * (lane >> 4), half8 = (lane >> 3) & 1;
         if constexpr (F8) {
           // chunk j holds head_dim 16 j ..: rows 2 i and 2 i + 1 of the result come from the low and the high byte of its pair i
 #pragma unroll
           for (int j = 0; j < kSteps; j += 2) {
-            if (j * 16 < dim) {
+            if (FULL || j * 16 < dim) {
               uint32_t r[4];   // chunk j, tokens 0-7; chunk j + 1, tokens 0-7; chunk j, tokens 8-15; chunk j + 1, tokens 8-15
-              ldmatrix_x4_trans(r, vs + chunk_at<S::kChunks>(tok, j + half8));
+              ldmatrix_x4_trans(r, vs + pair_at(v_at, u, j / 2));
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                if ((j + h) * 16 >= dim) break;
+                if (!FULL && (j + h) * 16 >= dim) break;
                 const uint32_t t0 = __byte_perm(r[h], 0, 0x3120), t1 = __byte_perm(r[h + 2], 0, 0x3120);
                 const uint32_t a[4] = {e4m3x2_to_f16x2(t0 & 0xFFFFu), e4m3x2_to_f16x2(t0 >> 16), e4m3x2_to_f16x2(t1 & 0xFFFFu), e4m3x2_to_f16x2(t1 >> 16)};
 #pragma unroll
@@ -425,9 +464,9 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
         } else {
 #pragma unroll
           for (int j = 0; j < kSteps; ++j) {
-            if (j * 16 < dim) {
+            if (FULL || j * 16 < dim) {
               uint32_t a[4];
-              ldmatrix_x4_trans(a, vs + chunk_at<S::kChunks>(tok, 2 * j + half8));
+              ldmatrix_x4_trans(a, vs + pair_at(v_at, u, j));
 #pragma unroll
               for (int n = 0; n < NT; ++n) mma_16816<kMmaBf16>(acc[j][n], a, pt[n][0], pt[n][1]);
             }
@@ -601,9 +640,9 @@ void launch_dependent(void (*kernel)(KArgs...), dim3 grid, size_t smem, cudaStre
   count_launch();
 }
 
-template <bool BF16, bool F8, int DP, int NT> void launch(PagedAttParams p, DeviceState &dev, cudaStream_t stream) {
+template <bool BF16, bool F8, int DP, int NT, bool FULL> void launch(PagedAttParams p, DeviceState &dev, cudaStream_t stream) {
   using S = Shape<F8, DP, NT>;
-  auto kernel = paged_attention_kernel<BF16, F8, DP, NT>;
+  auto kernel = paged_attention_kernel<BF16, F8, DP, NT, FULL>;
   static int resident[64] = {};   // blocks of an SM
   int &r = resident[dev.device & 63];
   if (!r) {
@@ -620,9 +659,12 @@ template <bool BF16, bool F8, int DP, int NT> void launch(PagedAttParams p, Devi
 
 template <bool BF16, bool F8> void launch(const PagedAttParams &p, int cols, DeviceState &dev, cudaStream_t stream) {
   const int dim = p.c.dim;
-  if (dim <= 64) cols == 16 ? launch<BF16, F8, 64, 2>(p, dev, stream) : launch<BF16, F8, 64, 1>(p, dev, stream);
-  else if (dim <= 128) cols == 16 ? launch<BF16, F8, 128, 2>(p, dev, stream) : launch<BF16, F8, 128, 1>(p, dev, stream);
-  else launch<BF16, F8, 256, 1>(p, dev, stream);
+  if (dim == 64) cols == 16 ? launch<BF16, F8, 64, 2, true>(p, dev, stream) : launch<BF16, F8, 64, 1, true>(p, dev, stream);
+  else if (dim < 64) cols == 16 ? launch<BF16, F8, 64, 2, false>(p, dev, stream) : launch<BF16, F8, 64, 1, false>(p, dev, stream);
+  else if (dim == 128) cols == 16 ? launch<BF16, F8, 128, 2, true>(p, dev, stream) : launch<BF16, F8, 128, 1, true>(p, dev, stream);
+  else if (dim < 128) cols == 16 ? launch<BF16, F8, 128, 2, false>(p, dev, stream) : launch<BF16, F8, 128, 1, false>(p, dev, stream);
+  else if (dim == 256) launch<BF16, F8, 256, 1, true>(p, dev, stream);
+  else launch<BF16, F8, 256, 1, false>(p, dev, stream);
 }
 
 } // namespace

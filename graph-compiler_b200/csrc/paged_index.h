@@ -17,14 +17,14 @@ struct PageTable {
   int sequences, max_pages, page_size, pages; // rows, entries of a row, tokens of a page, pages of the cache
 };
 
-// Page that holds position `pos` of sequence `seq`, or -1 when the table has no entry for it or the entry is outside the cache.
-GCB_HD int page_of(const PageTable &t, int seq, int pos) {
-  if (seq < 0 || seq >= t.sequences || pos < 0) return -1;
-  const int entry = pos / t.page_size;
-  if (entry >= t.max_pages) return -1;
+// Page in entry `entry` of sequence `seq`, or -1 when there is no such entry or it is outside the cache.
+GCB_HD int page_at(const PageTable &t, int seq, int entry) {
+  if (seq < 0 || seq >= t.sequences || entry < 0 || entry >= t.max_pages) return -1;
   const int page = t.entries[int64_t(seq) * t.stride + entry];
   return page >= 0 && page < t.pages ? page : -1;
 }
+// Page that holds position `pos`.
+GCB_HD int page_of(const PageTable &t, int seq, int pos) { return pos < 0 ? -1 : page_at(t, seq, pos / t.page_size); }
 
 // Positions [first, end) that a query sees in a sequence said to hold `length` tokens; window 0: all.  `cut`: length was more than
 // the table has room for.
