@@ -4,15 +4,23 @@
 // takes them: 1024 bytes of codes (lane l reads 16 bytes at 16 l of each half), the scales of the 16 outputs for each of the
 // block's groups, and their zeros.  The k range of an output tile is one contiguous stream.
 //
-// Codes become 16-bit floats without a conversion: four bits or-ed into the mantissa of 128 (bf16) or 1024 (f16) are that
-// number plus the code, and subtracting (128 or 1024) + zero is exact.  Products with X then are exact in f32, sums are f32, and
-// a group's scale multiplies the f32 sum of its products.
+// Codes become f16 numbers by a mask alone: four bits in the mantissa of a number with exponent zero are code * 2^-22 or
+// code * 2^-18 (a subnormal, exact).  A word of eight codes takes one byte permutation and four masks; one that went through
+// 16 + code took eight operations, and the integer units were what the kernel waited for.  With the sum of x over a group,
+// sum x (code - zero) = sum x code - zero sum x:  the zero costs one multiply-add per group and result.
+// X is f16 as it is; bf16 is scaled by a power of two per row and 128 k, which puts the largest magnitude at 2^14 and keeps
+// every bit down to 2^-38 of it.  Products are exact in f32, sums are f32, a group's scale multiplies its f32 sum.
 //
-// Bound by HBM: half a byte per weight.
+// Bound by HBM: half a byte per weight.  One block of sixteen warps to an SM stays there and works off its share of the output
+// tiles; every warp streams blocks of its own through a ring of bulk copies that runs on across the tiles.  X lies in shared
+// memory for the whole call.  Where it does not fit, or where there are fewer tiles than SMs, a cluster of 2 to 8 blocks shares
+// the k of its tiles and exchanges f32 sums through distributed shared memory, one tile late, so that nobody waits for them.
 #include "decode_ops.h"
 
 #include <algorithm>
+#include <mutex>
 #include <stdexcept>
+#include <type_traits>
 
 #include "mma_ptx.cuh"
 #include "runtime.h"
@@ -24,7 +32,7 @@ namespace {
 constexpr int kRows = 16;      // outputs of a tile: M of the matrix instruction
 constexpr int kBlockK = 128;
 constexpr int kCodes = kRows * kBlockK / 2;
-constexpr int kW4Warps = 8;
+constexpr int kW4Warps = 16;
 
 void require(bool ok, const char *what) {
   if (!ok) throw std::invalid_argument(what);
@@ -42,7 +50,9 @@ struct W4PackParams {
 };
 
 // One block of 256 threads packs one 16 x 128 block; a thread one 32-bit word.  Word w of a lane in half h covers
-// k = 64 h + 32 (w >> 1) + 8 c + 4 (w & 1) + {0, 1, 2, 3} of outputs r and r + 8 (r = lane / 4, c = lane % 4).
+// k = 64 h + 32 (w >> 1) + 8 c + 4 (w & 1) + {0, 1, 2, 3} of outputs r and r + 8 (r = lane / 4, c = lane % 4): the registers
+// s = 0..3 of the instruction's A operand, each a pair of k in the word's halves.  Within a half, code s lies where a mask finds
+// it: at bit 2, at bit 6, and, with the half's bytes exchanged, at bit 2 and bit 6 again.
 __global__ void __launch_bounds__(256) w4_pack_kernel(const __grid_constant__ W4PackParams p) {
   pdl_wait();
   pdl_launch_dependents();
@@ -52,96 +62,337 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const __grid_constant__ W4
   const int t = threadIdx.x, h = t >> 7, lane = (t >> 2) & 31, w = t & 3, r = lane >> 2, c = lane & 3;
   const int64_t k0 = kb * kBlockK + 64 * h + 32 * (w >> 1) + 8 * c + 4 * (w & 1);
   auto code = [&](int64_t n, int64_t k) -> uint32_t {
-    if (n >= p.N) return 8u;
-    if (k >= p.K) return p.zeros ? 0u : 8u;   // meets an x of zero
+    if (n >= p.N || k >= p.K) return 0u;   // meets a scale or an x of zero
     const uint32_t b = p.codes[n * p.codes_stride + (k >> 1)];
     return (k & 1) ? b >> 4 : b & 15u;
   };
   uint32_t word = 0;
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {   // nibbles s and s + 4: one register of the instruction's A operand
+  for (int s = 0; s < 4; ++s) {
     const int64_t n = nt * kRows + r + 8 * (s & 1), k = k0 + 2 * (s >> 1);
-    word |= code(n, k) << (4 * s) | code(n, k + 1) << (4 * s + 16);
+    const uint32_t pair = code(n, k) | code(n, k + 1) << 16;
+    word |= s < 3 ? pair << (4 * s + 2) : (pair & 0x00030003u) << 14 | (pair >> 2 & 0x00030003u);
   }
   reinterpret_cast<uint32_t *>(block)[h * 128 + lane * 4 + w] = word;
-  if (t < p.gpb * kRows) {
-    const int64_t n = nt * kRows + (t & 15), g = (kb * kBlockK + int64_t(t >> 4) * (kBlockK / p.gpb)) / p.group;
+  if (t < p.gpb * kRows) {   // [output][group]
+    const int64_t n = nt * kRows + t / p.gpb, g = (kb * kBlockK + int64_t(t % p.gpb) * (kBlockK / p.gpb)) / p.group;
     const bool in = n < p.N && g * p.group < p.K;
     reinterpret_cast<uint16_t *>(block + kCodes)[t] = in ? p.scales[n * p.scales_stride + g] : uint16_t(0);
-    if (p.zeros) block[kCodes + p.gpb * kRows * 2 + t] = in ? uint8_t(p.zeros[n * p.zeros_stride + g] & 15u) : uint8_t(8);
+    if (p.zeros) block[kCodes + p.gpb * kRows * 2 + t] = in ? uint8_t(p.zeros[n * p.zeros_stride + g] & 15u) : uint8_t(0);
   }
 }
+
+constexpr int kMaxStages = 8;
+constexpr int kXPad = 64;            // bytes behind a row of x: neighbouring rows lie 16 banks apart
+constexpr int kXMost = 96 * 1024;    // what x may have of a block's shared memory
 
 struct W4Params {
   const uint16_t *x, *bias;
   const uint8_t *packed;
   uint16_t *y;
-  int64_t ldx, ldy, N, K, kblocks;
-  int M, relu, bytes;
+  int64_t ldx, ldy, N, K;
+  int M, pass, relu, kblocks, tiles;   // pass: rows of x that a block takes; tiles: of 16 outputs
+  int cluster, share, wk, stages;      // blocks that share k; k blocks of each; warps of a block that share them; depth of a ring
+  int items;                           // groups of RT * (16 / wk) tiles
+  int x_at, table_at, meet_at, part_at;
+  int *error;
 };
 
-template <bool BF16> __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  if constexpr (BF16) asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+// Eight elements of x at `from`, of which the first `count` exist; [lo, hi): the bytes of all of x.  Rows on any two bytes: the two
+// aligned pieces around, where both lie inside x.
+__device__ __forceinline__ uint4 load_piece(const uint16_t *from, int64_t count, uintptr_t lo, uintptr_t hi) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(from), base = at & ~uintptr_t(15);
+  if (count >= 8 && at == base) return *reinterpret_cast<const uint4 *>(from);
+  if (count >= 8 && base >= lo && base + 32 <= hi) {
+    const uint4 u = *reinterpret_cast<const uint4 *>(base), v = *reinterpret_cast<const uint4 *>(base + 16);
+    uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+    const uint32_t off = uint32_t(at - base);
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+    const uint32_t bits = (off & 2) * 8;
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+  }
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < count) w[e >> 1] |= uint32_t(from[e]) << (16 * (e & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A block of eight warps per 16 outputs and 8 rows of x; the warps take every eighth k block and their sums meet in shared memory.
-template <bool BF16, int GPB, bool ZEROS>
-__global__ void __launch_bounds__(kW4Warps * 32) matmul_w4_kernel(const __grid_constant__ W4Params p) {
-  __shared__ float sums[kW4Warps][kRows][9];
+// RT tiles of 16 outputs to a warp, NT sets of 8 rows of x.
+template <bool BF16, int NT, int RT, int GPB, bool ZEROS>
+__global__ void __launch_bounds__(kW4Warps * 32, 1) matmul_w4_kernel(const __grid_constant__ W4Params p) {
+  constexpr int kBlock = kCodes + GPB * kRows * (ZEROS ? 3 : 2), kStage = RT * kBlock;
+  constexpr int kGroup = kBlockK / GPB, kThreads = kW4Warps * 32;
+  constexpr int kOuts = 16 * RT, kMeetRow = kOuts + 4, kMeet = 8 * NT * kMeetRow;   // floats; the pad keeps the columns' banks apart
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t full[kW4Warps][kMaxStages];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int wn = kW4Warps / p.wk, warp_n = warp / p.wk, warp_k = warp - warp_n * p.wk;
+  const int m0 = blockIdx.y * p.pass, rows = min(p.M - m0, p.pass);
+  const int cluster = int(blockIdx.x) / p.cluster, clusters = int(gridDim.x) / p.cluster, rank = int(blockIdx.x) - cluster * p.cluster;
+  const int kb0 = rank * p.share, here = max(0, min(p.share, p.kblocks - kb0));   // this block's k blocks
+  const int turns = warp_k < here ? (here - warp_k + p.wk - 1) / p.wk : 0;        // this warp's of each item
+  const int pitch = p.share * kBlockK * 2 + kXPad;
+  uint8_t *ring = smem + warp * p.stages * kStage, *x = smem + p.x_at;   // x: [rows + 1][pitch] f16, the last row zeros
+  float2 *table = reinterpret_cast<float2 *>(smem + p.table_at);         // [group][rows + 1]: sum of x, factor of the scaled x
+  float *meet = reinterpret_cast<float *>(smem + p.meet_at), *part = reinterpret_cast<float *>(smem + p.part_at);
+  if (lane == 0) {
+    for (int i = 0; i < p.stages; ++i) mbar_init(smem_u32(&full[warp][i]), 1);
+    mbar_fence_init();
+  }
+  __syncwarp();
   pdl_wait();
   pdl_launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int64_t nt = blockIdx.x;
-  const int m = blockIdx.y * 8 + r;
-  const uint32_t magic = BF16 ? 0x43004300u : 0x64006400u;
-  float acc[4] = {};
-  for (int64_t kb = warp; kb < p.kblocks; kb += kW4Warps) {
-    const uint8_t *block = p.packed + (nt * p.kblocks + kb) * p.bytes;
-    const uint16_t *scales = reinterpret_cast<const uint16_t *>(block + kCodes);
-    const uint8_t *zeros = block + kCodes + GPB * kRows * 2;
+
+  // ---- this warp's stream of weights: k blocks kb0 + warp_k, + wk, ... of its tiles of item `cluster`, + clusters, ...
+  const uint32_t ring_s = smem_u32(ring), bars_s = smem_u32(&full[warp][0]);
+  const int64_t tile_bytes = int64_t(p.kblocks) * kBlock, turn_bytes = int64_t(p.wk) * kBlock;
+  auto tiles_at = [&](int item) { return (item * wn + warp_n) * RT; };
+  int ask_item = cluster, ask_turn = 0, in_flight = 0;
+  const uint8_t *ask = p.packed + tiles_at(ask_item) * tile_bytes + int64_t(kb0 + warp_k) * kBlock;
+  auto issue = [&](int st) {   // the next block, if there is one
+    if (turns == 0 || ask_item >= p.items || tiles_at(ask_item) >= p.tiles) return;
+    if (lane == 0) {
+      const uint32_t bar = bars_s + st * 8, dst = ring_s + st * kStage;
+      const bool second = RT > 1 && tiles_at(ask_item) + 1 < p.tiles;
+      mbar_expect_tx(bar, second ? 2 * kBlock : kBlock);
+      bulk_load(dst, ask, kBlock, bar);
+      if (second) bulk_load(dst + kBlock, ask + tile_bytes, kBlock, bar);
+    }
+    ++in_flight;
+    ask += turn_bytes;
+    if (++ask_turn == turns) {
+      ask_turn = 0;
+      ask_item += clusters;
+      ask = p.packed + tiles_at(ask_item) * tile_bytes + int64_t(kb0 + warp_k) * kBlock;
+    }
+  };
+  for (int i = 0; i < p.stages; ++i) issue(i);
+
+  // ---- x into shared memory, sixteen lanes to a row's k block
+  {
+    const int row_pieces = p.share * (kBlockK / 8), pieces = rows * row_pieces;
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(p.x), hi = reinterpret_cast<uintptr_t>(p.x + (p.M - 1) * p.ldx + p.K);
+    for (int first = 0; first < pieces; first += kThreads) {
+      const int at = first + threadIdx.x, m = at / row_pieces, piece = at - m * row_pieces;
+      const int64_t k = int64_t(kb0) * kBlockK + piece * 8;
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (at < pieces && k < p.K) u = load_piece(p.x + (m0 + m) * p.ldx + k, p.K - k, lo, hi);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      float v[8], sum = 0.f, factor = 1.f;
 #pragma unroll
-    for (int g = 0; g < GPB; ++g) {
-      float part[4] = {};
-      const uint32_t z0 = magic + (ZEROS ? zeros[g * 16 + r] : 8u) * 0x10001u, z1 = magic + (ZEROS ? zeros[g * 16 + r + 8] : 8u) * 0x10001u;
-#pragma unroll
-      for (int s = g * 8 / GPB; s < (g + 1) * 8 / GPB; ++s) {   // sixteen k to a step
-        const uint32_t w = reinterpret_cast<const uint32_t *>(block)[(s >> 2) * 128 + lane * 4 + (s & 3)];
-        const int64_t k = kb * kBlockK + (s >> 1) * 32 + 8 * c + 4 * (s & 1);
-        uint32_t b[2] = {0u, 0u};
-        if (m < p.M) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (k + i < p.K) b[i >> 1] |= uint32_t(p.x[m * p.ldx + k + i]) << (16 * (i & 1));
-        }
-        const uint32_t a[4] = {sub2<BF16>((w & 0x000F000Fu) | magic, z0), sub2<BF16>(((w >> 4) & 0x000F000Fu) | magic, z1),
-                               sub2<BF16>(((w >> 8) & 0x000F000Fu) | magic, z0), sub2<BF16>(((w >> 12) & 0x000F000Fu) | magic, z1)};
-        mma_16816<BF16>(part, a, b[0], b[1]);
+      for (int e = 0; e < 8; ++e) {
+        v[e] = half_to_f32<BF16>((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu);
+        sum += v[e];
       }
-      const float s0 = half_to_f32<BF16>(scales[g * 16 + r]), s1 = half_to_f32<BF16>(scales[g * 16 + r + 8]);
-      acc[0] = fmaf(part[0], s0, acc[0]);
-      acc[1] = fmaf(part[1], s0, acc[1]);
-      acc[2] = fmaf(part[2], s1, acc[2]);
-      acc[3] = fmaf(part[3], s1, acc[3]);
+      if constexpr (BF16) {
+        float big = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(v[e]));
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
+        const int e2 = big < INFINITY ? max(int(__float_as_uint(big) >> 23) - 127 - 14, -110) : 0;   // big in [2^(e2 + 14), 2^(e2 + 15))
+        const float down = __uint_as_float(uint32_t(127 - e2) << 23);
+        factor = __uint_as_float(uint32_t(127 + e2) << 23);
+        u = make_uint4(pack_half2<false>(v[0] * down, v[1] * down), pack_half2<false>(v[2] * down, v[3] * down),
+                       pack_half2<false>(v[4] * down, v[5] * down), pack_half2<false>(v[6] * down, v[7] * down));
+      }
+#pragma unroll
+      for (int d = 1; d < kGroup / 8; d <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+      if (at < pieces) {
+        *reinterpret_cast<uint4 *>(x + m * pitch + piece * 16) = u;
+        if (piece % (kGroup / 8) == 0) table[piece / (kGroup / 8) * (rows + 1) + m] = make_float2(sum, factor);
+      }
+    }
+    for (int i = threadIdx.x; i < pitch / 16; i += kThreads) *reinterpret_cast<uint4 *>(x + rows * pitch + i * 16) = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < p.share * GPB; i += kThreads) table[i * (rows + 1) + rows] = make_float2(0.f, 0.f);
+  }
+  __syncthreads();
+
+  const int outs = kOuts * wn;   // of an item
+  auto store = [&](int item, int m, int o, float y) {
+    const int64_t n = int64_t(item) * outs + o;
+    if (n >= p.N) return;
+    if (p.bias) y += half_to_f32<BF16>(p.bias[n]);
+    if (p.relu) y = y != y ? y : fmaxf(y, 0.f);
+    p.y[(m0 + m) * p.ldy + n] = f32_to_half<BF16>(y);
+  };
+  // This block's share of an item whose parts all blocks of the cluster have written: sums in k order.
+  auto finish = [&](int item, int buffer) {
+    const int mine = outs / p.cluster, o0 = rank * mine;
+    const uint32_t base = smem_u32(part + buffer * 8 * NT * outs);
+    for (int i = threadIdx.x; i < rows * mine; i += kThreads) {
+      const int m = i / mine, o = o0 + i - m * mine;
+      float y = 0.f;
+      for (int q = 0; q < p.cluster; ++q) y += __uint_as_float(ld_shared_cluster(mapa_shared(base + uint32_t(m * outs + o) * 4u, uint32_t(q))));
+      store(item, m, o, y);
+    }
+  };
+
+  const uint8_t *xrow[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) xrow[n] = x + min(n * 8 + r, rows) * pitch + warp_k * kBlockK * 2 + c * 16;
+  const int x_turn = p.wk * kBlockK * 2, table_turn = p.wk * GPB * (rows + 1);
+  int st = 0, flip = 0, before = -1;
+  uint32_t parity = 0;
+  bool ok = true;
+  for (int item = cluster; item < p.items; item += clusters) {
+    float acc[RT][NT][4] = {};
+    const int todo = ok && tiles_at(item) < p.tiles ? turns : 0;
+    const uint8_t *xt[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) xt[n] = xrow[n];
+    const float2 *tab = table + warp_k * GPB * (rows + 1);
+    for (int turn = 0; turn < todo; ++turn) {
+      if (!mbar_wait(bars_s + st * 8, parity)) {
+        ok = false;
+        break;
+      }
+      const uint8_t *block = ring + st * kStage;
+      uint4 w4[RT][2];
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) w4[t][h] = *reinterpret_cast<const uint4 *>(block + t * kBlock + h * 512 + lane * 16);
+      // scales of outputs r and r + 8, all groups of the block
+      uint16_t scale[RT][2][GPB];
+      uint8_t zero[RT][2][GPB];
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint8_t *from = block + t * kBlock + kCodes + (r + 8 * h) * GPB * 2, *zfrom = block + t * kBlock + kCodes + GPB * kRows * 2 + (r + 8 * h) * GPB;
+          if constexpr (GPB == 1) {
+            scale[t][h][0] = *reinterpret_cast<const uint16_t *>(from);
+            if (ZEROS) zero[t][h][0] = *zfrom;
+          } else if constexpr (GPB == 2) {
+            const uint32_t u = *reinterpret_cast<const uint32_t *>(from);
+            scale[t][h][0] = uint16_t(u); scale[t][h][1] = uint16_t(u >> 16);
+            if (ZEROS) {
+              const uint16_t z = *reinterpret_cast<const uint16_t *>(zfrom);
+              zero[t][h][0] = uint8_t(z); zero[t][h][1] = uint8_t(z >> 8);
+            }
+          } else {
+            const uint2 u = *reinterpret_cast<const uint2 *>(from);
+            scale[t][h][0] = uint16_t(u.x); scale[t][h][1] = uint16_t(u.x >> 16);
+            scale[t][h][2] = uint16_t(u.y); scale[t][h][3] = uint16_t(u.y >> 16);
+            if (ZEROS) {
+              const uint32_t z = *reinterpret_cast<const uint32_t *>(zfrom);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) zero[t][h][i] = uint8_t(z >> (8 * i));
+            }
+          }
+        }
+#pragma unroll
+      for (int g = 0; g < GPB; ++g) {
+        float sum[RT][NT][4] = {};
+#pragma unroll
+        for (int q = g * 4 / GPB; q < (g + 1) * 4 / GPB; ++q) {   // 32 k
+          uint32_t b[NT][4];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(xt[n] + q * 64);
+            b[n][0] = u.x; b[n][1] = u.y; b[n][2] = u.z; b[n][3] = u.w;
+          }
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            const uint4 &u = w4[t][q >> 1];
+            const uint32_t w[2] = {q & 1 ? u.z : u.x, q & 1 ? u.w : u.y};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t v = __byte_perm(w[h], 0, 0x2301);
+              const uint32_t a[4] = {w[h] & 0x003C003Cu, w[h] & 0x03C003C0u, v & 0x003C003Cu, v & 0x03C003C0u};
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma_16816<false>(sum[t][n], a, b[n][2 * h], b[n][2 * h + 1]);
+            }
+          }
+        }
+        float2 xs[NT][2];   // columns 2 c and 2 c + 1
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) xs[n][i] = tab[g * (rows + 1) + min(n * 8 + 2 * c + i, rows)];
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float s = half_to_f32<BF16>(scale[t][h][g]);
+            const float z = ZEROS ? __uint_as_float(0x4B000000u | zero[t][h][g]) - 8388608.f : 8.f;
+            const float of_codes = s * (h ? 262144.f : 4194304.f), of_sum = -s * z;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const float v = BF16 ? sum[t][n][2 * h + i] * xs[n][i].y : sum[t][n][2 * h + i];
+                acc[t][n][2 * h + i] = fmaf(v, of_codes, fmaf(xs[n][i].x, of_sum, acc[t][n][2 * h + i]));
+              }
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) xt[n] += x_turn;
+      tab += table_turn;
+      __syncwarp();
+      --in_flight;
+      issue(st);
+      if (++st == p.stages) {
+        st = 0;
+        parity ^= 1u;
+      }
+    }
+    // ---- the warps' sums meet: [warp][rows of x][outputs]
+    float *at = meet + (NT == 1 ? flip * kW4Warps * kMeet : 0);
+    float *own = at + warp * kMeet;
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) own[(n * 8 + 2 * c + (i & 1)) * kMeetRow + t * 16 + r + 8 * (i >> 1)] = acc[t][n][i];
+    __syncthreads();
+    if (p.cluster > 1 && before >= 0) {   // the item before: everybody's part is there
+      cluster_wait();
+      finish(before, flip ^ 1);
+    }
+    for (int i = threadIdx.x; i < rows * outs; i += kThreads) {
+      const int m = i / outs, o = i - m * outs, w0 = o / kOuts * p.wk;
+      const float *from = at + w0 * kMeet + m * kMeetRow + o % kOuts;
+      float y = 0.f;
+      for (int w = 0; w < p.wk; ++w) y += from[w * kMeet];
+      if (p.cluster > 1) part[(flip * 8 * NT + m) * outs + o] = y;
+      else store(item, m, o, y);
+    }
+    if (p.cluster > 1) cluster_arrive();
+    if (NT > 1) __syncthreads();   // one buffer: before the next item writes there
+    flip ^= 1;
+    before = item;
+  }
+  if (!ok) {   // a copy never arrived: say so, and leave with nothing in flight
+    if (lane == 0) atomicExch(p.error, int(ERR_WAIT_FULL));
+    for (int i = 1; i < in_flight; ++i) {   // the stages behind the one that failed
+      if (++st == p.stages) {
+        st = 0;
+        parity ^= 1u;
+      }
+      if (!mbar_wait(bars_s + st * 8, parity) && lane == 0) atomicExch(p.error, int(ERR_WAIT_DRAIN));
     }
   }
-  sums[warp][r][2 * c] = acc[0];
-  sums[warp][r][2 * c + 1] = acc[1];
-  sums[warp][r + 8][2 * c] = acc[2];
-  sums[warp][r + 8][2 * c + 1] = acc[3];
-  __syncthreads();
-  if (threadIdx.x < 128) {
-    const int row = threadIdx.x & 15, col = threadIdx.x >> 4, out_m = blockIdx.y * 8 + col;
-    const int64_t n = nt * kRows + row;
-    if (n < p.N && out_m < p.M) {
-      float y = 0.f;
-      for (int w = 0; w < kW4Warps; ++w) y += sums[w][row][col];
-      if (p.bias) y += half_to_f32<BF16>(p.bias[n]);
-      if (p.relu) y = y != y ? y : fmaxf(y, 0.f);
-      p.y[out_m * p.ldy + n] = f32_to_half<BF16>(y);
+  if (p.cluster > 1) {
+    if (before >= 0) {
+      cluster_wait();
+      finish(before, flip ^ 1);
     }
+    cluster_arrive();   // nobody leaves while others read its parts
+    cluster_wait();
   }
 }
 
@@ -150,12 +401,113 @@ void checked_w4(int64_t N, int64_t K, int64_t group) {
   require(group == 32 || group == 64 || (group > 0 && group % kBlockK == 0), "4-bit weights: group must be 32, 64 or a multiple of 128");
 }
 
-template <bool BF16> void launch(const W4Params &p, int gpb, bool zeros, dim3 grid, cudaStream_t stream) {
-  auto go = [&](auto kernel) { kernel<<<grid, kW4Warps * 32, 0, stream>>>(p); };
-  if (zeros) gpb == 1 ? go(matmul_w4_kernel<BF16, 1, true>) : gpb == 2 ? go(matmul_w4_kernel<BF16, 2, true>) : go(matmul_w4_kernel<BF16, 4, true>);
-  else gpb == 1 ? go(matmul_w4_kernel<BF16, 1, false>) : gpb == 2 ? go(matmul_w4_kernel<BF16, 2, false>) : go(matmul_w4_kernel<BF16, 4, false>);
-  GCB_CUDA(cudaGetLastError());
-  count_launch();
+// How a call is shared out.
+struct W4Plan {
+  int pass, nt, rt, cluster, share, wk, clusters, stages;
+  int x_at, table_at, meet_at, part_at, smem;
+};
+constexpr int kMostSmem = 225 * 1024;
+
+template <bool BF16, int NT, int RT, int GPB, bool ZEROS> struct W4Kernel {
+  static void configure(cudaLaunchConfig_t &cfg, cudaLaunchAttribute (&at)[2], int grid_x, int grid_y, int cluster, size_t smem, cudaStream_t stream) {
+    cfg = {};
+    cfg.gridDim = dim3(unsigned(grid_x), unsigned(grid_y), 1u);
+    cfg.blockDim = dim3(kW4Warps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = unsigned(cluster);
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+  }
+  static void run(const W4Params &p, const W4Plan &plan, int grid_y, int device, cudaStream_t stream) {
+    static bool ready[64] = {};
+    auto kernel = matmul_w4_kernel<BF16, NT, RT, GPB, ZEROS>;
+    if (!ready[device & 63]) {
+      GCB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem));
+      ready[device & 63] = true;
+    }
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute at[2];
+    configure(cfg, at, plan.cluster * plan.clusters, grid_y, plan.cluster, size_t(plan.smem), stream);
+    GCB_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+    count_launch();
+  }
+};
+
+template <bool BF16, int NT, int RT> void launch(const W4Params &p, const W4Plan &plan, int gpb, bool zeros, int grid_y, int device, cudaStream_t stream) {
+  if (zeros) gpb == 1 ? W4Kernel<BF16, NT, RT, 1, true>::run(p, plan, grid_y, device, stream) : gpb == 2 ? W4Kernel<BF16, NT, RT, 2, true>::run(p, plan, grid_y, device, stream)
+                                                                                                         : W4Kernel<BF16, NT, RT, 4, true>::run(p, plan, grid_y, device, stream);
+  else gpb == 1 ? W4Kernel<BF16, NT, RT, 1, false>::run(p, plan, grid_y, device, stream) : gpb == 2 ? W4Kernel<BF16, NT, RT, 2, false>::run(p, plan, grid_y, device, stream)
+                                                                                                    : W4Kernel<BF16, NT, RT, 4, false>::run(p, plan, grid_y, device, stream);
+}
+
+// Clusters of each size that a device runs at the same time, one block to an SM.
+const int *clusters_at_once(const DeviceState &dev) {
+  struct State {
+    std::once_flag once;
+    int at_once[9] = {};
+  };
+  static State states[64];
+  State &s = states[dev.device & 63];
+  std::call_once(s.once, [&] {
+    using Kernel = W4Kernel<true, 1, 2, 1, false>;
+    auto kernel = matmul_w4_kernel<true, 1, 2, 1, false>;
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
+    s.at_once[1] = dev.sm_count;
+    for (int n = 2; n <= 8; n *= 2) {
+      cudaLaunchConfig_t cfg;
+      cudaLaunchAttribute at[2];
+      Kernel::configure(cfg, at, n, 1, n, kMostSmem, nullptr);
+      int k = 0;
+      if (cudaOccupancyMaxActiveClusters(&k, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        k = 0;
+      }
+      s.at_once[n] = k;
+    }
+  });
+  return s.at_once;
+}
+
+int up(int v, int step) { return (v + step - 1) / step * step; }
+
+// The fastest way by a rough model: an SM takes 0.17 us for the sixteen blocks of 1 KB that its warps work on at a time (what
+// HBM gives it), an item costs 0.25 us beyond its blocks and an exchange in the cluster as much again.
+bool plan_w4(int M, int tiles, int kblocks, int gpb, int bytes, const int *at_once, W4Plan *best) {
+  double cost = 1e30;
+  for (int pass = std::min(M, 16); pass >= 1 && cost == 1e30; pass = pass > 8 ? 8 : pass / 2) {   // fewer rows at a time only where x does not fit
+    const int nt = pass > 8 ? 2 : 1;
+    for (int cluster = 1; cluster <= 8; cluster *= 2) {
+      const int share = (kblocks + cluster - 1) / cluster;
+      if (at_once[cluster] < 1 || cluster > kblocks || (pass + 1) * (share * kBlockK * 2 + kXPad) > kXMost) continue;
+      for (int rt = 1; rt <= 2; ++rt)
+        for (int wk = 1; wk <= kW4Warps; wk *= 2) {
+          const int per_item = rt * (kW4Warps / wk), items = (tiles + per_item - 1) / per_item;
+          W4Plan p{pass, nt, rt, cluster, share, wk, std::min(at_once[cluster], items), 0, 0, 0, 0, 0, 0};
+          const int outs = 16 * per_item, turns = (share + wk - 1) / wk, rounds = (items + p.clusters - 1) / p.clusters;
+          const int x = up((pass + 1) * (share * kBlockK * 2 + kXPad), 128), table = up((pass + 1) * share * gpb * 8, 128);
+          const int meet = up((nt == 1 ? 2 : 1) * kW4Warps * 8 * nt * (16 * rt + 4) * 4, 128), part = cluster > 1 ? 2 * 8 * nt * outs * 4 : 0;
+          const int stage = kW4Warps * rt * bytes, room = (kMostSmem - x - table - meet - part) / stage;
+          if (room < 2) continue;
+          p.stages = std::max(1, std::min({kMaxStages, room, turns * rounds}));
+          p.x_at = up(p.stages * stage, 128);
+          p.table_at = p.x_at + x;
+          p.meet_at = p.table_at + table;
+          p.part_at = p.meet_at + meet;
+          p.smem = p.part_at + part;
+          const double us = rounds * (turns * rt * 0.17 * 2 + 0.25 * (cluster > 1 ? 2 : 1)) + 1e-3 * pass * share;
+          if (us < cost) {
+            cost = us;
+            *best = p;
+          }
+        }
+    }
+  }
+  return cost < 1e30;
 }
 
 } // namespace
@@ -201,23 +553,44 @@ void matmul_w4(int dtype, const void *X, int64_t ldx, const void *packed, const 
   require(X && packed && Y, "4-bit weights: null pointer");
   require((reinterpret_cast<uintptr_t>(packed) & 15) == 0, "4-bit weights: the packed buffer must be 16-byte aligned");
   require(M == 1 || (ldx >= K && ldy >= N), "4-bit weights: rows overlap");
-  device_state();
+  DeviceState &dev = device_state();
+  const int kblocks = int((K + kBlockK - 1) / kBlockK), tiles = int((N + kRows - 1) / kRows);
+  const int gpb = groups_per_block(group), bytes = block_bytes(group, has_zeros != 0);
+  W4Plan plan{};
+  if (!plan_w4(int(M), tiles, kblocks, gpb, bytes, clusters_at_once(dev), &plan)) throw std::logic_error("4-bit weights: a row of x does not fit into the shared memory of a cluster");
   W4Params p{};
   p.x = static_cast<const uint16_t *>(X);
   p.bias = static_cast<const uint16_t *>(bias);
   p.packed = static_cast<const uint8_t *>(packed);
   p.y = static_cast<uint16_t *>(Y);
-  p.ldx = ldx;
-  p.ldy = ldy;
+  p.ldx = M > 1 ? ldx : 0;
+  p.ldy = M > 1 ? ldy : 0;
   p.N = N;
   p.K = K;
-  p.kblocks = (K + kBlockK - 1) / kBlockK;
   p.M = int(M);
+  p.pass = plan.pass;
   p.relu = relu;
-  p.bytes = block_bytes(group, has_zeros != 0);
-  const dim3 grid(unsigned((N + kRows - 1) / kRows), unsigned((M + 7) / 8));
-  if (dtype == GCB200_BF16) launch<true>(p, groups_per_block(group), has_zeros != 0, grid, stream);
-  else launch<false>(p, groups_per_block(group), has_zeros != 0, grid, stream);
+  p.kblocks = kblocks;
+  p.tiles = tiles;
+  p.cluster = plan.cluster;
+  p.share = plan.share;
+  p.wk = plan.wk;
+  p.stages = plan.stages;
+  const int per_item = plan.rt * (kW4Warps / plan.wk);
+  p.items = (tiles + per_item - 1) / per_item;
+  p.x_at = plan.x_at;
+  p.table_at = plan.table_at;
+  p.meet_at = plan.meet_at;
+  p.part_at = plan.part_at;
+  p.error = dev.d_error;
+  const int grid_y = int((M + plan.pass - 1) / plan.pass);
+  require(grid_y <= 65535, "4-bit weights: number of rows out of range");
+  auto go = [&](auto bf16) {
+    constexpr bool B = decltype(bf16)::value;
+    if (plan.nt == 1) plan.rt == 2 ? launch<B, 1, 2>(p, plan, gpb, has_zeros != 0, grid_y, dev.device, stream) : launch<B, 1, 1>(p, plan, gpb, has_zeros != 0, grid_y, dev.device, stream);
+    else plan.rt == 2 ? launch<B, 2, 2>(p, plan, gpb, has_zeros != 0, grid_y, dev.device, stream) : launch<B, 2, 1>(p, plan, gpb, has_zeros != 0, grid_y, dev.device, stream);
+  };
+  dtype == GCB200_BF16 ? go(std::true_type{}) : go(std::false_type{});
 }
 
 } // namespace gcb

@@ -35,7 +35,6 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kStages = 3;
 constexpr int kMaxBlocks = 592;   // the workspace has two parts for each
 constexpr float kLazy = 8.f;
 
@@ -59,6 +58,11 @@ template <bool F8, int DP, int NT> struct Shape {
   static constexpr int kTile = kWarps * kTokens;
   static constexpr int kSlot = 2 * kTokens * kRow;          // a warp's keys and values of one tile
   static constexpr int kCols = 8 * NT;                      // query heads
+#ifdef GCB_ST
+  static constexpr int kStages = GCB_ST;
+#else
+  static constexpr int kStages = 3;
+#endif
   static constexpr int kQRow = DP * 2 + 16;                 // bytes, padded against bank conflicts
   static constexpr int kQ = kCols * kQRow;
   static constexpr int kBytes = kStages * kWarps * kSlot + (kStages + 1) * kQ;
@@ -158,7 +162,7 @@ template <bool BF16, bool F8, int DP, int NT, bool FULL>
 __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_constant__ PagedAttParams p) {
   using S = Shape<F8, DP, NT>;
   constexpr bool kMmaBf16 = BF16 && !F8;
-  constexpr int kSteps = DP / 16, kSubs = S::kTokens / 16;
+  constexpr int kStages = S::kStages, kSteps = DP / 16, kSubs = S::kTokens / 16;
   constexpr float kBelow = kMmaBf16 ? 0.f : 7.f;   // the reference under the maximum: P reaches 2^(kBelow + kLazy), below f16's 2^16
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t pre[kThreads + 1];
