@@ -8,13 +8,14 @@
 // code * 2^-18 (a subnormal, exact).  A word of eight codes takes one byte permutation and four masks; one that went through
 // 16 + code took eight operations, and the integer units were what the kernel waited for.  With the sum of x over a group,
 // sum x (code - zero) = sum x code - zero sum x:  the zero costs one multiply-add per group and result.
-// X is f16 as it is; bf16 is scaled by a power of two per row and 128 k, which puts the largest magnitude at 2^14 and keeps
-// every bit down to 2^-38 of it.  Products are exact in f32, sums are f32, a group's scale multiplies its f32 sum.
+// X is f16 as it is; bf16 is scaled by a power of two per row and 128 k, which puts the largest magnitude at 2^14 and drops
+// nothing above 2^-38 of it.  Products are exact in f32, sums are f32, a group's scale multiplies its f32 sum.
 //
 // Bound by HBM: half a byte per weight.  One block of sixteen warps to an SM stays there and works off its share of the output
-// tiles; every warp streams blocks of its own through a ring of bulk copies that runs on across the tiles.  X lies in shared
+// tiles; every warp streams blocks of its own through a ring of asynchronous copies that runs on across the tiles.  X lies in shared
 // memory for the whole call.  Where it does not fit, or where there are fewer tiles than SMs, a cluster of 2 to 8 blocks shares
 // the k of its tiles and exchanges f32 sums through distributed shared memory, one tile late, so that nobody waits for them.
+// (1 KB bulk copies instead of the warps' 16-byte ones kept an SM at 12 to 20 bytes a cycle, half of what HBM gives it.)
 #include "decode_ops.h"
 
 #include <algorithm>
@@ -32,7 +33,7 @@ namespace {
 constexpr int kRows = 16;      // outputs of a tile: M of the matrix instruction
 constexpr int kBlockK = 128;
 constexpr int kCodes = kRows * kBlockK / 2;
-constexpr int kW4Warps = 16;
+constexpr int kW4Warps = 16, kSumWarps = 4, kW4Threads = (kW4Warps + kSumWarps) * 32;
 
 void require(bool ok, const char *what) {
   if (!ok) throw std::invalid_argument(what);
@@ -82,7 +83,7 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const __grid_constant__ W4
   }
 }
 
-constexpr int kMaxStages = 8;
+constexpr int kMaxStages = 4;
 constexpr int kXPad = 64;            // bytes behind a row of x: neighbouring rows lie 16 banks apart
 constexpr int kXMost = 96 * 1024;    // what x may have of a block's shared memory
 
@@ -93,17 +94,9 @@ struct W4Params {
   int64_t ldx, ldy, N, K;
   int M, pass, relu, kblocks, tiles;   // pass: rows of x that a block takes; tiles: of 16 outputs
   int cluster, share, wk, stages;      // blocks that share k; k blocks of each; warps of a block that share them; depth of a ring
-  int items;                           // groups of RT * (16 / wk) tiles
   int x_at, table_at, meet_at, part_at;
   int *error;
 };
-
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // Eight elements of x at `from`, of which the first `count` exist; [lo, hi): the bytes of all of x.  Rows on any two bytes: the two
 // aligned pieces around, where both lie inside x.
@@ -128,271 +121,360 @@ __device__ __forceinline__ uint4 load_piece(const uint16_t *from, int64_t count,
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// RT tiles of 16 outputs to a warp, NT sets of 8 rows of x.
+struct W4Bars {
+  uint64_t meet_full, meet_empty;      // the warps' sums of an item are there / have been read
+  uint64_t parts_in[2], parts_out[2];  // the cluster's sums of an item are there / have been read by everyone
+};
+__device__ __forceinline__ float4 ld_shared_cluster_v4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
+  return v;
+}
+// Bounded waits of the adding warps, which wait most of the time: asleep, off the issue slots of the warps that multiply.
+template <bool CLUSTER> __device__ __forceinline__ bool wait_asleep(uint32_t bar, uint32_t parity) {
+  auto there = [&] { return CLUSTER ? mbar_test_cluster(bar, parity) : mbar_test(bar, parity); };
+  const long long t0 = clock64();
+  while (!__all_sync(0xFFFFFFFFu, there())) {
+    if (__any_sync(0xFFFFFFFFu, clock64() - t0 > WAIT_LIMIT_CYCLES)) return false;
+    __nanosleep(100);
+  }
+  return true;
+}
+__device__ __forceinline__ void complain(int *error, bool ok, int code) {
+  if (!ok && lane_id() == 0) atomicExch(error, code);
+}
+
+// RT tiles of 16 outputs to a warp, NT sets of 8 rows of x.  Warps 0-15 multiply, each with a stream of weights of its own; warps
+// 16-19 add up and store.  Nobody waits for all the others.
 template <bool BF16, int NT, int RT, int GPB, bool ZEROS>
-__global__ void __launch_bounds__(kW4Warps * 32, 1) matmul_w4_kernel(const __grid_constant__ W4Params p) {
+__global__ void __launch_bounds__(kW4Threads, 1) matmul_w4_kernel(const __grid_constant__ W4Params p) {
   constexpr int kBlock = kCodes + GPB * kRows * (ZEROS ? 3 : 2), kStage = RT * kBlock;
-  constexpr int kGroup = kBlockK / GPB, kThreads = kW4Warps * 32;
+  constexpr int kGroup = kBlockK / GPB, kMulThreads = kW4Warps * 32;
+  constexpr float kUnit = 1.f / 4194304.f;   // of the codes of outputs r; of outputs r + 8 it is 16 times that
   constexpr int kOuts = 16 * RT, kMeetRow = kOuts + 4, kMeet = 8 * NT * kMeetRow;   // floats; the pad keeps the columns' banks apart
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t full[kW4Warps][kMaxStages];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int wn = kW4Warps / p.wk, warp_n = warp / p.wk, warp_k = warp - warp_n * p.wk;
+  __shared__ W4Bars bars;
+  const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x >> 5), 0);   // known to be the same in all lanes
+  const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int wn = kW4Warps / p.wk;
   const int m0 = blockIdx.y * p.pass, rows = min(p.M - m0, p.pass);
   const int cluster = int(blockIdx.x) / p.cluster, clusters = int(gridDim.x) / p.cluster, rank = int(blockIdx.x) - cluster * p.cluster;
   const int kb0 = rank * p.share, here = max(0, min(p.share, p.kblocks - kb0));   // this block's k blocks
-  const int turns = warp_k < here ? (here - warp_k + p.wk - 1) / p.wk : 0;        // this warp's of each item
-  const int pitch = p.share * kBlockK * 2 + kXPad;
-  uint8_t *ring = smem + warp * p.stages * kStage, *x = smem + p.x_at;   // x: [rows + 1][pitch] f16, the last row zeros
-  float2 *table = reinterpret_cast<float2 *>(smem + p.table_at);         // [group][rows + 1]: sum of x, factor of the scaled x
+  const int pitch = p.share * kBlockK * 2 + kXPad, outs = kOuts * wn;             // outs: outputs of an item
+  uint8_t *x = smem + p.x_at;   // [rows + 1][pitch] f16, the last row zeros
+  // [group][rows + 1]: factor of the scaled x, and -2^-22 sum of the scaled x (times 8 where that is the zero of all)
+  float2 *table = reinterpret_cast<float2 *>(smem + p.table_at);
   float *meet = reinterpret_cast<float *>(smem + p.meet_at), *part = reinterpret_cast<float *>(smem + p.part_at);
-  if (lane == 0) {
-    for (int i = 0; i < p.stages; ++i) mbar_init(smem_u32(&full[warp][i]), 1);
+  const uint32_t meet_full = smem_u32(&bars.meet_full), meet_empty = smem_u32(&bars.meet_empty);
+  if (threadIdx.x == 0) {
+    mbar_init(meet_full, kW4Warps);
+    mbar_init(meet_empty, kSumWarps);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bars.parts_in[i]), uint32_t(p.cluster * kSumWarps));
+      mbar_init(smem_u32(&bars.parts_out[i]), uint32_t(p.cluster * kSumWarps));
+    }
     mbar_fence_init();
   }
-  __syncwarp();
+  __syncthreads();
+  if (p.cluster > 1) cluster_sync_all();   // every block's barriers are there before another one signals them
   pdl_wait();
   pdl_launch_dependents();
+  // A cluster's tiles, an equal share of all, in items of wn RT; warp w multiplies k blocks kb0 + w % wk, + wk, ... of RT of them.
+  const int first = int(int64_t(p.tiles) * cluster / clusters), last = int(int64_t(p.tiles) * (cluster + 1) / clusters);
+  const int items = (last - first + wn * RT - 1) / (wn * RT);
+  auto tile_of = [&](int w, int item) { return first + (item * wn + w / p.wk) * RT; };
 
-  // ---- this warp's stream of weights: k blocks kb0 + warp_k, + wk, ... of its tiles of item `cluster`, + clusters, ...
-  const uint32_t ring_s = smem_u32(ring), bars_s = smem_u32(&full[warp][0]);
-  const int64_t tile_bytes = int64_t(p.kblocks) * kBlock, turn_bytes = int64_t(p.wk) * kBlock;
-  auto tiles_at = [&](int item) { return (item * wn + warp_n) * RT; };
-  int ask_item = cluster, ask_turn = 0, in_flight = 0;
-  const uint8_t *ask = p.packed + tiles_at(ask_item) * tile_bytes + int64_t(kb0 + warp_k) * kBlock;
-  auto issue = [&](int st) {   // the next block, if there is one
-    if (turns == 0 || ask_item >= p.items || tiles_at(ask_item) >= p.tiles) return;
-    if (lane == 0) {
-      const uint32_t bar = bars_s + st * 8, dst = ring_s + st * kStage;
-      const bool second = RT > 1 && tiles_at(ask_item) + 1 < p.tiles;
-      mbar_expect_tx(bar, second ? 2 * kBlock : kBlock);
-      bulk_load(dst, ask, kBlock, bar);
-      if (second) bulk_load(dst + kBlock, ask + tile_bytes, kBlock, bar);
-    }
-    ++in_flight;
-    ask += turn_bytes;
-    if (++ask_turn == turns) {
-      ask_turn = 0;
-      ask_item += clusters;
-      ask = p.packed + tiles_at(ask_item) * tile_bytes + int64_t(kb0 + warp_k) * kBlock;
-    }
-  };
-  for (int i = 0; i < p.stages; ++i) issue(i);
-
-  // ---- x into shared memory, sixteen lanes to a row's k block
-  {
-    const int row_pieces = p.share * (kBlockK / 8), pieces = rows * row_pieces;
-    const uintptr_t lo = reinterpret_cast<uintptr_t>(p.x), hi = reinterpret_cast<uintptr_t>(p.x + (p.M - 1) * p.ldx + p.K);
-    for (int first = 0; first < pieces; first += kThreads) {
-      const int at = first + threadIdx.x, m = at / row_pieces, piece = at - m * row_pieces;
-      const int64_t k = int64_t(kb0) * kBlockK + piece * 8;
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (at < pieces && k < p.K) u = load_piece(p.x + (m0 + m) * p.ldx + k, p.K - k, lo, hi);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-      float v[8], sum = 0.f, factor = 1.f;
+  if (warp >= kW4Warps) {
+    // ------------------------------------------------------------------ sums of the warps and of the cluster, results
+    const int thread = threadIdx.x - kW4Warps * 32;
+    const int64_t n_end = min(p.N, int64_t(last) * kRows);
+    auto store = [&](int item, int m, int o, const float (&v)[4], int count) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[e] = half_to_f32<BF16>((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu);
-        sum += v[e];
+      for (int i = 0; i < 4; ++i) {
+        const int64_t n = int64_t(first) * kRows + int64_t(item) * outs + o + i;
+        if (i >= count || n >= n_end) break;
+        float y = v[i];
+        if (p.bias) y += half_to_f32<BF16>(p.bias[n]);
+        if (p.relu) y = y != y ? y : fmaxf(y, 0.f);
+        p.y[(m0 + m) * p.ldy + n] = f32_to_half<BF16>(y);
       }
-      if constexpr (BF16) {
-        float big = 0.f;
+    };
+    const int mine = outs / p.cluster;                         // outputs of an item that this block finishes
+    auto signal = [&](uint64_t *bar) {                         // to every block of the cluster, by one lane each
+      __syncwarp();
+      if (lane < p.cluster) mbar_arrive_cluster(mapa_shared(smem_u32(bar), uint32_t(lane)));
+    };
+    bool ok = true;
+    auto finish = [&](int item, int use) {   // use: which item of this block, in order
+      const int buffer = use & 1;
+      ok = wait_asleep<true>(smem_u32(&bars.parts_in[buffer]), uint32_t(use >> 1) & 1u) && ok;
+      const uint32_t base = smem_u32(part + buffer * 8 * NT * outs);
+      const int per = (mine + 3) / 4;   // fours of a row; `mine` may be 2
+      for (int i = thread; i < rows * per; i += kSumWarps * 32) {
+        const int m = i / per, o = rank * mine + (i - m * per) * 4;
+        const uint32_t at = base + uint32_t(m * outs + (o & ~3)) * 4u;
+        float4 f[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(v[e]));
+        for (int q = 0; q < 8; ++q)
+          if (q < p.cluster) f[q] = ld_shared_cluster_v4(mapa_shared(at, uint32_t(q)));
+        float v[4] = {};
 #pragma unroll
-        for (int d = 1; d < 16; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
-        const int e2 = big < INFINITY ? max(int(__float_as_uint(big) >> 23) - 127 - 14, -110) : 0;   // big in [2^(e2 + 14), 2^(e2 + 15))
-        const float down = __uint_as_float(uint32_t(127 - e2) << 23);
-        factor = __uint_as_float(uint32_t(127 + e2) << 23);
-        u = make_uint4(pack_half2<false>(v[0] * down, v[1] * down), pack_half2<false>(v[2] * down, v[3] * down),
-                       pack_half2<false>(v[4] * down, v[5] * down), pack_half2<false>(v[6] * down, v[7] * down));
+        for (int q = 0; q < 8; ++q)   // in k order
+          if (q < p.cluster) {
+            v[0] += f[q].x; v[1] += f[q].y; v[2] += f[q].z; v[3] += f[q].w;
+          }
+        if (o & 3) {   // two outputs to a block, the second pair of a four
+          v[0] = v[2];
+          v[1] = v[3];
+        }
+        store(item, m, o, v, mine);
       }
-#pragma unroll
-      for (int d = 1; d < kGroup / 8; d <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-      if (at < pieces) {
-        *reinterpret_cast<uint4 *>(x + m * pitch + piece * 16) = u;
-        if (piece % (kGroup / 8) == 0) table[piece / (kGroup / 8) * (rows + 1) + m] = make_float2(sum, factor);
+      signal(&bars.parts_out[buffer]);
+    };
+    int use = 0, before = -1;
+    for (int item = 0; item < items; ++item, ++use) {
+      ok = wait_asleep<false>(meet_full, uint32_t(use) & 1u) && ok;
+      const int buffer = use & 1;
+      if (p.cluster > 1 && use >= 2) ok = wait_asleep<true>(smem_u32(&bars.parts_out[buffer]), uint32_t((use >> 1) - 1) & 1u) && ok;
+      for (int i = thread; i < rows * (outs / 4); i += kSumWarps * 32) {
+        const int m = i / (outs / 4), o = (i - m * (outs / 4)) * 4;
+        const float *at = meet + o / kOuts * p.wk * kMeet + m * kMeetRow + o % kOuts;
+        float v[4] = {};
+#pragma unroll 4
+        for (int w = 0; w < p.wk; ++w) {
+          const float4 f = *reinterpret_cast<const float4 *>(at + w * kMeet);
+          v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
+        }
+        if (p.cluster > 1) *reinterpret_cast<float4 *>(part + (buffer * 8 * NT + m) * outs + o) = make_float4(v[0], v[1], v[2], v[3]);
+        else store(item, m, o, v, 4);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(meet_empty);
+      if (p.cluster > 1) {
+        signal(&bars.parts_in[buffer]);
+        if (before >= 0) finish(before, use - 1);   // one item late: everybody's part has come meanwhile
+        before = item;
       }
     }
-    for (int i = threadIdx.x; i < pitch / 16; i += kThreads) *reinterpret_cast<uint4 *>(x + rows * pitch + i * 16) = make_uint4(0, 0, 0, 0);
-    for (int i = threadIdx.x; i < p.share * GPB; i += kThreads) table[i * (rows + 1) + rows] = make_float2(0.f, 0.f);
-  }
-  __syncthreads();
-
-  const int outs = kOuts * wn;   // of an item
-  auto store = [&](int item, int m, int o, float y) {
-    const int64_t n = int64_t(item) * outs + o;
-    if (n >= p.N) return;
-    if (p.bias) y += half_to_f32<BF16>(p.bias[n]);
-    if (p.relu) y = y != y ? y : fmaxf(y, 0.f);
-    p.y[(m0 + m) * p.ldy + n] = f32_to_half<BF16>(y);
-  };
-  // This block's share of an item whose parts all blocks of the cluster have written: sums in k order.
-  auto finish = [&](int item, int buffer) {
-    const int mine = outs / p.cluster, o0 = rank * mine;
-    const uint32_t base = smem_u32(part + buffer * 8 * NT * outs);
-    for (int i = threadIdx.x; i < rows * mine; i += kThreads) {
-      const int m = i / mine, o = o0 + i - m * mine;
-      float y = 0.f;
-      for (int q = 0; q < p.cluster; ++q) y += __uint_as_float(ld_shared_cluster(mapa_shared(base + uint32_t(m * outs + o) * 4u, uint32_t(q))));
-      store(item, m, o, y);
-    }
-  };
-
-  const uint8_t *xrow[NT];
+    if (before >= 0) finish(before, use - 1);
+    complain(p.error, ok, ERR_WAIT_PARTS);
+  } else {
+    // ------------------------------------------------------------------ this warp's stream of weights
+    const int warp_k = warp % p.wk, turns = max(0, (here - warp_k + p.wk - 1) / p.wk);
+    const int64_t tile_bytes = int64_t(p.kblocks) * kBlock, turn_bytes = int64_t(p.wk) * kBlock;
+    uint8_t *ring = smem + warp * p.stages * kStage;
+    const uint32_t ring_s = smem_u32(ring) + lane * 16;
+    int ask_item = 0, ask_turn = 0, ask_tiles = 0;
+    const uint8_t *ask = nullptr;
+    auto ask_next = [&]() {
+      const int tile = tile_of(warp, ask_item);
+      ask_turn = turns;
+      ask_tiles = turns > 0 && ask_item < items ? max(0, min(RT, last - tile)) : 0;
+      ask = p.packed + tile * tile_bytes + int64_t(kb0 + warp_k) * kBlock + lane * 16;
+      ++ask_item;
+    };
+    auto issue = [&](int st) {   // the next block, if there is one
+      if (ask_tiles > 0) {
 #pragma unroll
-  for (int n = 0; n < NT; ++n) xrow[n] = x + min(n * 8 + r, rows) * pitch + warp_k * kBlockK * 2 + c * 16;
-  const int x_turn = p.wk * kBlockK * 2, table_turn = p.wk * GPB * (rows + 1);
-  int st = 0, flip = 0, before = -1;
-  uint32_t parity = 0;
-  bool ok = true;
-  for (int item = cluster; item < p.items; item += clusters) {
-    float acc[RT][NT][4] = {};
-    const int todo = ok && tiles_at(item) < p.tiles ? turns : 0;
-    const uint8_t *xt[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) xt[n] = xrow[n];
-    const float2 *tab = table + warp_k * GPB * (rows + 1);
-    for (int turn = 0; turn < todo; ++turn) {
-      if (!mbar_wait(bars_s + st * 8, parity)) {
-        ok = false;
-        break;
-      }
-      const uint8_t *block = ring + st * kStage;
-      uint4 w4[RT][2];
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) w4[t][h] = *reinterpret_cast<const uint4 *>(block + t * kBlock + h * 512 + lane * 16);
-      // scales of outputs r and r + 8, all groups of the block
-      uint16_t scale[RT][2][GPB];
-      uint8_t zero[RT][2][GPB];
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint8_t *from = block + t * kBlock + kCodes + (r + 8 * h) * GPB * 2, *zfrom = block + t * kBlock + kCodes + GPB * kRows * 2 + (r + 8 * h) * GPB;
-          if constexpr (GPB == 1) {
-            scale[t][h][0] = *reinterpret_cast<const uint16_t *>(from);
-            if (ZEROS) zero[t][h][0] = *zfrom;
-          } else if constexpr (GPB == 2) {
-            const uint32_t u = *reinterpret_cast<const uint32_t *>(from);
-            scale[t][h][0] = uint16_t(u); scale[t][h][1] = uint16_t(u >> 16);
-            if (ZEROS) {
-              const uint16_t z = *reinterpret_cast<const uint16_t *>(zfrom);
-              zero[t][h][0] = uint8_t(z); zero[t][h][1] = uint8_t(z >> 8);
-            }
-          } else {
-            const uint2 u = *reinterpret_cast<const uint2 *>(from);
-            scale[t][h][0] = uint16_t(u.x); scale[t][h][1] = uint16_t(u.x >> 16);
-            scale[t][h][2] = uint16_t(u.y); scale[t][h][3] = uint16_t(u.y >> 16);
-            if (ZEROS) {
-              const uint32_t z = *reinterpret_cast<const uint32_t *>(zfrom);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) zero[t][h][i] = uint8_t(z >> (8 * i));
-            }
+        for (int t = 0; t < RT; ++t) {
+          if (t < ask_tiles) {
+            const uint32_t dst = ring_s + st * kStage + t * kBlock;
+            const uint8_t *from = ask + t * tile_bytes;
+            cp_async_16(dst, from, 16);
+            cp_async_16(dst + 512, from + 512, 16);
+            if (lane * 16 < kBlock - kCodes) cp_async_16(dst + 1024, from + 1024, 16);
           }
         }
+        ask += turn_bytes;
+        if (--ask_turn == 0) ask_next();
+      }
+      cp_async_commit();
+    };
+    auto arrived = [&]() {   // the oldest block asked for
+      if (p.stages == 4) cp_async_wait<3>();
+      else if (p.stages == 3) cp_async_wait<2>();
+      else cp_async_wait<1>();
+      __syncwarp();
+    };
+    ask_next();
+    for (int i = 0; i < p.stages; ++i) issue(i);
+    // ------------------------------------------------------------------ x into shared memory, a warp to two k blocks of a row
+    {
+      const uintptr_t lo = reinterpret_cast<uintptr_t>(p.x), hi = reinterpret_cast<uintptr_t>(p.x + (p.M - 1) * p.ldx + p.K);
+      const int row_pairs = (p.share + 1) / 2, pieces = p.share * (kBlockK / 8);
+      constexpr int kBatch = 4;   // loads under way at a time
+      int m = 0, pair = warp;
+      while (m < rows) {
+        uint4 held[kBatch];
+        int row[kBatch], piece[kBatch];
 #pragma unroll
-      for (int g = 0; g < GPB; ++g) {
-        float sum[RT][NT][4] = {};
-#pragma unroll
-        for (int q = g * 4 / GPB; q < (g + 1) * 4 / GPB; ++q) {   // 32 k
-          uint32_t b[NT][4];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint4 u = *reinterpret_cast<const uint4 *>(xt[n] + q * 64);
-            b[n][0] = u.x; b[n][1] = u.y; b[n][2] = u.z; b[n][3] = u.w;
+        for (int b = 0; b < kBatch; ++b) {
+          while (m < rows && pair >= row_pairs) {
+            pair -= row_pairs;
+            ++m;
           }
+          row[b] = m;
+          piece[b] = pair * 32 + lane;
+          const int64_t k = int64_t(kb0) * kBlockK + piece[b] * 8;
+          held[b] = make_uint4(0, 0, 0, 0);
+          if (m < rows && piece[b] < pieces && k < p.K) held[b] = load_piece(p.x + (m0 + m) * p.ldx + k, p.K - k, lo, hi);
+          pair += kW4Warps;
+        }
 #pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            const uint4 &u = w4[t][q >> 1];
-            const uint32_t w[2] = {q & 1 ? u.z : u.x, q & 1 ? u.w : u.y};
+        for (int b = 0; b < kBatch; ++b) {
+          if (row[b] >= rows) break;
+          uint4 u = held[b];
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+          float down = 1.f, factor = 1.f;
+          if constexpr (BF16) {
+            // magnitudes compare like their bits; the largest of the k block lies in [2^(e + 14), 2^(e + 15))
+            uint32_t big2 = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu), __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t v = __byte_perm(w[h], 0, 0x2301);
-              const uint32_t a[4] = {w[h] & 0x003C003Cu, w[h] & 0x03C003C0u, v & 0x003C003Cu, v & 0x03C003C0u};
+            for (int d = 1; d < 16; d <<= 1) big2 = __vmaxu2(big2, __shfl_xor_sync(0xFFFFFFFFu, big2, d));
+            const int field = int(max(big2 & 0xFFFFu, big2 >> 16) >> 7), e = field == 255 ? 0 : max(field - 127 - 14, -110);
+            down = __uint_as_float(uint32_t(127 - e) << 23);
+            factor = __uint_as_float(uint32_t(127 + e) << 23);
+          }
+          float v[8];
 #pragma unroll
-              for (int n = 0; n < NT; ++n) mma_16816<false>(sum[t][n], a, b[n][2 * h], b[n][2 * h + 1]);
-            }
+          for (int e = 0; e < 8; ++e) v[e] = half_to_f32<BF16>((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu) * down;
+          float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+          if constexpr (BF16) u = make_uint4(pack_half2<false>(v[0], v[1]), pack_half2<false>(v[2], v[3]), pack_half2<false>(v[4], v[5]), pack_half2<false>(v[6], v[7]));
+#pragma unroll
+          for (int d = 1; d < kGroup / 8; d <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+          if (piece[b] < pieces) {
+            *reinterpret_cast<uint4 *>(x + row[b] * pitch + piece[b] * 16) = u;
+            if (lane % (kGroup / 8) == 0) table[piece[b] / (kGroup / 8) * (rows + 1) + row[b]] = make_float2(factor, sum * (ZEROS ? -kUnit : -8.f * kUnit));
           }
         }
-        float2 xs[NT][2];   // columns 2 c and 2 c + 1
+      }
+      for (int i = threadIdx.x; i < pitch / 16; i += kMulThreads) *reinterpret_cast<uint4 *>(x + rows * pitch + i * 16) = make_uint4(0, 0, 0, 0);
+      for (int i = threadIdx.x; i < p.share * GPB; i += kMulThreads) table[i * (rows + 1) + rows] = make_float2(0.f, 0.f);
+      asm volatile("bar.sync 1, %0;" ::"n"(kMulThreads) : "memory");
+    }
+    // ------------------------------------------------------------------ products
+    const uint8_t *xrow[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) xrow[n] = x + min(n * 8 + r, rows) * pitch + warp_k * kBlockK * 2 + c * 16;
+    const int col0 = min(2 * c, rows), col1 = min(2 * c + 1, rows), col2 = min(2 * c + 8, rows), col3 = min(2 * c + 9, rows);
+    const int x_turn = p.wk * kBlockK * 2, table_turn = (p.wk - 1) * GPB * (rows + 1);
+    float *own = meet + warp * kMeet + 2 * c * kMeetRow + r;
+    int st = 0;
+    uint32_t meet_parity = 1;   // the first item finds the place free
+    bool ok = true;
+    for (int item = 0; item < items; ++item) {
+      float acc[RT][NT][4] = {};
+      const int todo = tile_of(warp, item) < last ? turns : 0;
+      const uint8_t *xt[NT];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) xs[n][i] = tab[g * (rows + 1) + min(n * 8 + 2 * c + i, rows)];
+      for (int n = 0; n < NT; ++n) xt[n] = xrow[n];
+      const float2 *tab = table + warp_k * GPB * (rows + 1);
+#pragma unroll 1
+      for (int turn = 0; turn < todo; ++turn) {
+        arrived();
+        const uint8_t *block = ring + st * kStage;
+        uint4 w4[RT][2];
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) w4[t][h] = *reinterpret_cast<const uint4 *>(block + t * kBlock + h * 512 + lane * 16);
+        // scales of outputs r and r + 8, all groups of the block
+        uint32_t scale[RT][2][(GPB + 1) / 2], zero[RT][2];
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float s = half_to_f32<BF16>(scale[t][h][g]);
-            const float z = ZEROS ? __uint_as_float(0x4B000000u | zero[t][h][g]) - 8388608.f : 8.f;
-            const float of_codes = s * (h ? 262144.f : 4194304.f), of_sum = -s * z;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const float v = BF16 ? sum[t][n][2 * h + i] * xs[n][i].y : sum[t][n][2 * h + i];
-                acc[t][n][2 * h + i] = fmaf(v, of_codes, fmaf(xs[n][i].x, of_sum, acc[t][n][2 * h + i]));
-              }
+            const uint8_t *from = block + t * kBlock + kCodes + (r + 8 * h) * GPB * 2, *zfrom = block + t * kBlock + kCodes + GPB * kRows * 2 + (r + 8 * h) * GPB;
+            if constexpr (GPB == 1) {
+              scale[t][h][0] = *reinterpret_cast<const uint16_t *>(from);
+              zero[t][h] = ZEROS ? *zfrom : 0u;
+            } else if constexpr (GPB == 2) {
+              scale[t][h][0] = *reinterpret_cast<const uint32_t *>(from);
+              zero[t][h] = ZEROS ? *reinterpret_cast<const uint16_t *>(zfrom) : 0u;
+            } else {
+              const uint2 u = *reinterpret_cast<const uint2 *>(from);
+              scale[t][h][0] = u.x;
+              scale[t][h][1] = u.y;
+              zero[t][h] = ZEROS ? *reinterpret_cast<const uint32_t *>(zfrom) : 0u;
+            }
           }
-      }
+        __syncwarp();
+        issue(st);   // all of the stage is in registers
 #pragma unroll
-      for (int n = 0; n < NT; ++n) xt[n] += x_turn;
-      tab += table_turn;
+        for (int g = 0; g < GPB; ++g) {
+          float sum[RT][NT][4];
+          // in units of the codes:  acc += scale factor (sum x code - zero sum x);  the second term is what the products start from
+          float2 xs[NT][2];   // columns 2 c and 2 c + 1
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            xs[n][0] = tab[n ? col2 : col0];
+            xs[n][1] = tab[n ? col3 : col1];
+          }
+          tab += rows + 1;
+#pragma unroll
+          for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float z = ZEROS ? (__uint_as_float(0x4B000000u | ((zero[t][h] >> (8 * g)) & 0xFFu)) - 8388608.f) * (h ? 16.f : 1.f) : (h ? 16.f : 1.f);
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) sum[t][n][2 * h + i] = xs[n][i].y * z;
+            }
+#pragma unroll
+          for (int q = g * 4 / GPB; q < (g + 1) * 4 / GPB; ++q) {   // 32 k
+            uint32_t b[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const uint4 u = *reinterpret_cast<const uint4 *>(xt[n] + q * 64);
+              b[n][0] = u.x; b[n][1] = u.y; b[n][2] = u.z; b[n][3] = u.w;
+            }
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+              const uint4 &u = w4[t][q >> 1];
+              const uint32_t w[2] = {q & 1 ? u.z : u.x, q & 1 ? u.w : u.y};
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t v = __byte_perm(w[h], 0, 0x2301);
+                const uint32_t a[4] = {w[h] & 0x003C003Cu, w[h] & 0x03C003C0u, v & 0x003C003Cu, v & 0x03C003C0u};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma_16816<false>(sum[t][n], a, b[n][2 * h], b[n][2 * h + 1]);
+              }
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float s = half_to_f32<BF16>((scale[t][h][g / 2] >> (16 * (g & 1))) & 0xFFFFu);
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) acc[t][n][2 * h + i] = fmaf(BF16 ? sum[t][n][2 * h + i] * xs[n][i].x : sum[t][n][2 * h + i], s, acc[t][n][2 * h + i]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) xt[n] += x_turn;
+        tab += table_turn;
+        if (++st == p.stages) st = 0;
+      }
+      // ---- [warp][rows of x][outputs]
+      if (!mbar_wait(meet_empty, meet_parity)) ok = false;
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) own[(n * 8 + (i & 1)) * kMeetRow + t * 16 + 8 * (i >> 1)] = acc[t][n][i] * (i >> 1 ? 0.0625f / kUnit : 1.f / kUnit);
       __syncwarp();
-      --in_flight;
-      issue(st);
-      if (++st == p.stages) {
-        st = 0;
-        parity ^= 1u;
-      }
+      if (lane == 0) mbar_arrive(meet_full);
+      meet_parity ^= 1u;
     }
-    // ---- the warps' sums meet: [warp][rows of x][outputs]
-    float *at = meet + (NT == 1 ? flip * kW4Warps * kMeet : 0);
-    float *own = at + warp * kMeet;
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) own[(n * 8 + 2 * c + (i & 1)) * kMeetRow + t * 16 + r + 8 * (i >> 1)] = acc[t][n][i];
-    __syncthreads();
-    if (p.cluster > 1 && before >= 0) {   // the item before: everybody's part is there
-      cluster_wait();
-      finish(before, flip ^ 1);
-    }
-    for (int i = threadIdx.x; i < rows * outs; i += kThreads) {
-      const int m = i / outs, o = i - m * outs, w0 = o / kOuts * p.wk;
-      const float *from = at + w0 * kMeet + m * kMeetRow + o % kOuts;
-      float y = 0.f;
-      for (int w = 0; w < p.wk; ++w) y += from[w * kMeet];
-      if (p.cluster > 1) part[(flip * 8 * NT + m) * outs + o] = y;
-      else store(item, m, o, y);
-    }
-    if (p.cluster > 1) cluster_arrive();
-    if (NT > 1) __syncthreads();   // one buffer: before the next item writes there
-    flip ^= 1;
-    before = item;
-  }
-  if (!ok) {   // a copy never arrived: say so, and leave with nothing in flight
-    if (lane == 0) atomicExch(p.error, int(ERR_WAIT_FULL));
-    for (int i = 1; i < in_flight; ++i) {   // the stages behind the one that failed
-      if (++st == p.stages) {
-        st = 0;
-        parity ^= 1u;
-      }
-      if (!mbar_wait(bars_s + st * 8, parity) && lane == 0) atomicExch(p.error, int(ERR_WAIT_DRAIN));
-    }
+    complain(p.error, ok, ERR_WAIT_EMPTY);
   }
   if (p.cluster > 1) {
-    if (before >= 0) {
-      cluster_wait();
-      finish(before, flip ^ 1);
-    }
-    cluster_arrive();   // nobody leaves while others read its parts
-    cluster_wait();
+    __syncwarp();
+    cluster_sync_all();   // nobody leaves while others read its sums
   }
 }
 
@@ -406,13 +488,13 @@ struct W4Plan {
   int pass, nt, rt, cluster, share, wk, clusters, stages;
   int x_at, table_at, meet_at, part_at, smem;
 };
-constexpr int kMostSmem = 225 * 1024;
+constexpr int kMostSmem = 223 * 1024;
 
 template <bool BF16, int NT, int RT, int GPB, bool ZEROS> struct W4Kernel {
   static void configure(cudaLaunchConfig_t &cfg, cudaLaunchAttribute (&at)[2], int grid_x, int grid_y, int cluster, size_t smem, cudaStream_t stream) {
     cfg = {};
     cfg.gridDim = dim3(unsigned(grid_x), unsigned(grid_y), 1u);
-    cfg.blockDim = dim3(kW4Warps * 32);
+    cfg.blockDim = dim3(kW4Threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -475,8 +557,12 @@ const int *clusters_at_once(const DeviceState &dev) {
 
 int up(int v, int step) { return (v + step - 1) / step * step; }
 
-// The fastest way by a rough model: an SM takes 0.17 us for the sixteen blocks of 1 KB that its warps work on at a time (what
-// HBM gives it), an item costs 0.25 us beyond its blocks and an exchange in the cluster as much again.
+// The fastest way by a model fitted to all ways of twelve shapes.  An SM works off 42 KB of weights a microsecond (near HBM's
+// rate), 34 with more than four rows of x and 22 with more than eight, where the products of two instructions' columns and the
+// loads of x take most of the issue slots; a warp alone needs 0.15 us for a block.  On top: 15 ns for a turn of the warps, 0.1 us
+// for an item, 0.3 where a cluster exchanges its sums, 1 us for a cluster of 2 or 4 and 4 for one of 8 (fewer find room), 8 ns for
+// every row and k block of x.  Measured, the plan it takes against the fastest of all: 1 x 28672 x 8192 26.2 us (25.6), 8 rows 34.9
+// (31.3), 16 rows 46.2 (44.6); 1 x 4096 x 4096 6.0 (5.9), 16 rows 10.6 (10.4); 5 x 11001 x 4095, groups of 32, 13.7 (13.5).
 bool plan_w4(int M, int tiles, int kblocks, int gpb, int bytes, const int *at_once, W4Plan *best) {
   double cost = 1e30;
   for (int pass = std::min(M, 16); pass >= 1 && cost == 1e30; pass = pass > 8 ? 8 : pass / 2) {   // fewer rows at a time only where x does not fit
@@ -488,18 +574,21 @@ bool plan_w4(int M, int tiles, int kblocks, int gpb, int bytes, const int *at_on
         for (int wk = 1; wk <= kW4Warps; wk *= 2) {
           const int per_item = rt * (kW4Warps / wk), items = (tiles + per_item - 1) / per_item;
           W4Plan p{pass, nt, rt, cluster, share, wk, std::min(at_once[cluster], items), 0, 0, 0, 0, 0, 0};
-          const int outs = 16 * per_item, turns = (share + wk - 1) / wk, rounds = (items + p.clusters - 1) / p.clusters;
+          const int outs = 16 * per_item, turns = (share + wk - 1) / wk, most = (tiles + p.clusters - 1) / p.clusters;
           const int x = up((pass + 1) * (share * kBlockK * 2 + kXPad), 128), table = up((pass + 1) * share * gpb * 8, 128);
-          const int meet = up((nt == 1 ? 2 : 1) * kW4Warps * 8 * nt * (16 * rt + 4) * 4, 128), part = cluster > 1 ? 2 * 8 * nt * outs * 4 : 0;
+          const int meet = up(kW4Warps * 8 * nt * (16 * rt + 4) * 4, 128), part = cluster > 1 ? 2 * 8 * nt * outs * 4 : 0;
           const int stage = kW4Warps * rt * bytes, room = (kMostSmem - x - table - meet - part) / stage;
           if (room < 2) continue;
-          p.stages = std::max(1, std::min({kMaxStages, room, turns * rounds}));
+          p.stages = std::min(kMaxStages, room);
           p.x_at = up(p.stages * stage, 128);
           p.table_at = p.x_at + x;
           p.meet_at = p.table_at + table;
           p.part_at = p.meet_at + meet;
           p.smem = p.part_at + part;
-          const double us = rounds * (turns * rt * 0.17 * 2 + 0.25 * (cluster > 1 ? 2 : 1)) + 1e-3 * pass * share;
+          const double rate = (pass > 8 ? 22e3 : pass > 4 ? 34e3 : 42e3) * (rt == 2 && pass > 2 ? 0.96 : 1.0);   // two tiles at a time: fewer registers to spare
+          const int full = most / per_item, rest = most - full * per_item;
+          const double us = turns * (full * per_item * wk * bytes / rate + (rest ? std::max(rest * wk * bytes / rate, rt * 0.15) : 0.0)) +
+                            (full + (rest > 0)) * ((cluster > 1 ? 0.3 : 0.1) + 0.015 * turns) + (cluster > 4 ? 4.0 : cluster > 1 ? 1.0 : 0.0) + 0.008 * pass * share;
           if (us < cost) {
             cost = us;
             *best = p;
@@ -576,8 +665,6 @@ void matmul_w4(int dtype, const void *X, int64_t ldx, const void *packed, const 
   p.share = plan.share;
   p.wk = plan.wk;
   p.stages = plan.stages;
-  const int per_item = plan.rt * (kW4Warps / plan.wk);
-  p.items = (tiles + per_item - 1) / per_item;
   p.x_at = plan.x_at;
   p.table_at = plan.table_at;
   p.meet_at = plan.meet_at;
