@@ -61,7 +61,7 @@ template <bool F8, int DP, int NT> struct Shape {
 #ifdef GCB_ST
   static constexpr int kStages = GCB_ST;
 #else
-  static constexpr int kStages = 3;
+  static constexpr int kStages = F8 && DP >= 128 ? 2 : 3;
 #endif
   static constexpr int kQRow = DP * 2 + 16;                 // bytes, padded against bank conflicts
   static constexpr int kQ = kCols * kQRow;
@@ -170,7 +170,8 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
   __shared__ float stat_m[kWarps][S::kCols], stat_l[kWarps][S::kCols];
 
   const PagedCache &c = p.c;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row8 = lane >> 2, col4 = lane & 3;
+  const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x >> 5), 0);   // known to be the same in all lanes
+  const int lane = threadIdx.x & 31, row8 = lane >> 2, col4 = lane & 3;
   const int units = c.kv_heads * p.sets, dim = FULL ? DP : c.dim;
   pdl_wait();
   pdl_launch_dependents();   // behind the wait: what starts now finds everything before this kernel done
