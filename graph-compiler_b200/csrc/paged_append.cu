@@ -20,7 +20,7 @@ namespace gcb {
 
 namespace {
 
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 128;
 constexpr int kMaxDim = 256;
 
 struct AppendParams {
@@ -75,84 +75,60 @@ template <bool BF16, int VEC> __device__ __forceinline__ Chunk<VEC> pack(const f
   for (int i = 0; i < (VEC + 1) / 2; ++i) c.w[i] = pack_half2<BF16>(x[2 * i], VEC > 1 ? x[VEC > 1 ? 2 * i + 1 : 0] : 0.f);
   return c;
 }
-// 8-bit codes of x / scale.  The quotient is a true division: a product with the reciprocal would round twice.
-template <int VEC, bool ALIGNED> __device__ __forceinline__ void store_e4m3(uint8_t *p, const float (&x)[VEC], float scale) {
+// 8-bit codes of x times `by`, the reciprocal of the scale: a quotient within 2^-23 of the border between two codes may go to the
+// other one (a division takes four times the instructions of all the rest).
+template <int VEC, bool ALIGNED> __device__ __forceinline__ void store_e4m3(uint8_t *p, const float (&x)[VEC], float by) {
   if constexpr (ALIGNED) {
     uint32_t w[VEC / 4];
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i)
-      w[i] = f32x2_to_e4m3x2(__fdiv_rn(x[4 * i], scale), __fdiv_rn(x[4 * i + 1], scale)) |
-             (f32x2_to_e4m3x2(__fdiv_rn(x[4 * i + 2], scale), __fdiv_rn(x[4 * i + 3], scale)) << 16);
+      w[i] = f32x2_to_e4m3x2(x[4 * i] * by, x[4 * i + 1] * by) | (f32x2_to_e4m3x2(x[4 * i + 2] * by, x[4 * i + 3] * by) << 16);
     if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t *>(p) = w[0];
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) p[i] = uint8_t(f32x2_to_e4m3x2(__fdiv_rn(x[i], scale), 0.f));
+    for (int i = 0; i < VEC; ++i) p[i] = uint8_t(f32x2_to_e4m3x2(x[i] * by, 0.f));
   }
 }
 
-// A thread's piece of a row: two chunks of VEC elements, the partners of a rotation by halves or neighbours.
-struct Piece {
-  const uint16_t *src;
-  uint16_t *dst;
-  float scale;
-  int d0, d1;          // first elements of the chunks; d1 may lie behind the row
-  bool live, cached, rotated, partners;
-};
-template <bool F8, int VEC> __device__ __forceinline__ Piece piece_of(const AppendParams &p, int u, int64_t t, int page, int slot) {
-  const PagedCache &c = p.c;
-  Piece x;
-  const int q_rows = p.q ? p.heads : 0, row = u / p.units, half = p.rotary >> 1;
-  int i = u - row * p.units;
-  x.live = row < q_rows + 2 * c.kv_heads;
-  x.cached = row >= q_rows;
-  x.rotated = p.rotary > 0;
-  x.scale = 1.f;
-  x.src = nullptr;
-  x.dst = nullptr;
-  if (!x.cached) {
-    x.src = p.q + t * p.q_token + row * p.q_head;
-    x.dst = p.q_out + t * p.o_token + row * p.o_head;
-  } else if (x.live && page >= 0) {
-    const int r = row - q_rows, head = r < c.kv_heads ? r : r - c.kv_heads;
-    if (r < c.kv_heads) {
-      x.src = p.k + t * p.k_token + head * p.k_head;
-      x.dst = reinterpret_cast<uint16_t *>(c.keys + page * c.key_page + head * c.key_head + slot * c.key_token);
-      if (F8 && c.key_scale) x.scale = c.key_scale[head];
-    } else {
-      x.src = p.v + t * p.v_token + head * p.v_head;
-      x.dst = reinterpret_cast<uint16_t *>(c.values + page * c.value_page + head * c.value_head + slot * c.value_token);
-      if (F8 && c.value_scale) x.scale = c.value_scale[head];
-      x.rotated = false;
-    }
-  } else {
-    x.live = false;
-  }
-  const bool halves = x.rotated && !p.interleaved;
-  x.partners = halves && i * VEC < half;
-  if (x.partners) {
-    x.d0 = i * VEC;
-    x.d1 = x.d0 + half;
-  } else {
-    if (halves) i -= half / VEC;
-    x.d0 = (halves ? p.rotary : 0) + 2 * i * VEC;
-    x.d1 = x.d0 + VEC;
-  }
-  if (x.d0 >= c.dim) x.live = false;
-  return x;
-}
-
-// One block per token.
+// One block per token.  A thread has the same piece of every row it takes - two chunks of VEC elements, the partners of a rotation by
+// halves or neighbours - so that it loads its cosines and sines once; it takes rows kBatch at a time and asks for all of them, the
+// first ones before the angles are there.
 template <bool BF16, bool F8, int VEC, bool ALIGNED>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendParams p) {
   __shared__ float2 turn[kMaxDim / 2];   // (cos, sin) of each pair
   pdl_wait();
   pdl_launch_dependents();
   const PagedCache &c = p.c;
-  const int t = blockIdx.x;
-  const int seq = p.sequences ? p.sequences[t] : t, pos = p.positions[t];
+  const int64_t t = blockIdx.x;
+  const int seq = p.sequences ? p.sequences[t] : int(t), pos = p.positions[t];
   if (seq < 0 || pos < 0) return;   // padding
-  const int half = p.rotary >> 1;
+
+  const int half = p.rotary >> 1, q_rows = p.q ? p.heads : 0, rows = q_rows + 2 * c.kv_heads;
+  const int row_step = kAppendThreads / p.units, row0 = int(threadIdx.x) / p.units, piece = int(threadIdx.x) - row0 * p.units;
+  // Where the piece lies in a rotated row and in a row that is only copied.
+  const bool halves = p.rotary > 0 && !p.interleaved, partners = halves && piece * VEC < half;
+  const int rot0 = partners ? piece * VEC : halves ? p.rotary + 2 * (piece - half / VEC) * VEC : 2 * piece * VEC, rot1 = rot0 + (partners ? half : VEC);
+  const int copy0 = 2 * piece * VEC, copy1 = copy0 + VEC;
+
+  constexpr int kBatch = 4;
+  Chunk<VEC> a[kBatch], b[kBatch];
+  auto fetch = [&](int first) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int row = first + i * row_step;
+      if (row0 < row_step && row < rows) {
+        const bool copied = row >= q_rows + c.kv_heads;
+        const uint16_t *src = row < q_rows ? p.q + t * p.q_token + row * p.q_head
+                              : copied     ? p.v + t * p.v_token + (row - q_rows - c.kv_heads) * p.v_head
+                                           : p.k + t * p.k_token + (row - q_rows) * p.k_head;
+        const int d0 = copied ? copy0 : rot0, d1 = copied ? copy1 : rot1;
+        if (d0 < c.dim) a[i] = load<VEC, ALIGNED>(src + d0);
+        if (d1 < c.dim) b[i] = load<VEC, ALIGNED>(src + d1);
+      }
+    }
+  };
+  fetch(row0);
   for (int i = threadIdx.x; i < half; i += kAppendThreads) {
     const double turns = double(pos) * p.inv_freq[i] * 0.15915494309189533577;   // 1 / (2 pi)
     float s, co;
@@ -162,66 +138,90 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
   const int slot = pos % c.table.page_size, page = page_of(c.table, seq, pos);
   if (page < 0 && threadIdx.x == 0) atomicExch(c.error, int(ERR_BAD_PAGE));
   __syncthreads();
+  // this piece's pairs: element i of one chunk and of the other, or neighbours within a chunk
+  float cs[VEC], sn[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    const int at = partners ? rot0 + i : ((i < VEC / 2 ? rot0 : rot1) >> 1) + (VEC > 1 ? i % ((VEC + 1) / 2) : 0);
+    const float2 w = turn[partners || (p.interleaved && at < half) ? at : 0];   // unused where the piece does not turn
+    cs[i] = w.x;
+    sn[i] = w.y;
+  }
+  const bool turns = partners || (p.rotary > 0 && p.interleaved);
 
-  const int rows = (p.q ? p.heads : 0) + 2 * c.kv_heads;
-  for (int u = threadIdx.x; u < rows * p.units; u += kAppendThreads) {
-    const Piece x = piece_of<F8, VEC>(p, u, t, page, slot);
-    if (!x.live) continue;
-    const bool both = x.d1 < c.dim;
-    Chunk<VEC> ca = load<VEC, ALIGNED>(x.src + x.d0), cb = ca;
-    if (both) cb = load<VEC, ALIGNED>(x.src + x.d1);
-    if (x.rotated || (F8 && x.cached)) {
-      float a[VEC], b[VEC];
-      unpack<BF16, VEC>(ca, a);
-      unpack<BF16, VEC>(cb, b);
-      if (x.partners) {
+  for (int first = row0; first < rows; first += kBatch * row_step) {
+    if (first != row0) fetch(first);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float2 w = turn[x.d0 + i];
-          const float f = a[i], g = b[i];
-          a[i] = f * w.x - g * w.y;
-          b[i] = g * w.x + f * w.y;
-        }
-      } else if (x.rotated && p.interleaved) {
-        if constexpr (VEC >= 2) {
+    for (int i = 0; i < kBatch; ++i) {
+      const int row = first + i * row_step;
+      if (row0 >= row_step || row >= rows) continue;
+      const bool cached = row >= q_rows, copied = row >= q_rows + c.kv_heads;
+      if (cached && page < 0) continue;
+      const int d0 = copied ? copy0 : rot0, d1 = copied ? copy1 : rot1, head = copied ? row - q_rows - c.kv_heads : row - q_rows;
+      uint8_t *dst = !cached ? reinterpret_cast<uint8_t *>(p.q_out + t * p.o_token + row * p.o_head)
+                     : copied ? c.values + page * c.value_page + head * c.value_head + slot * c.value_token
+                              : c.keys + page * c.key_page + head * c.key_head + slot * c.key_token;
+      Chunk<VEC> ca = a[i], cb = b[i];
+      if ((turns && !copied) || (F8 && cached)) {
+        float x[VEC], y[VEC];
+        unpack<BF16, VEC>(ca, x);
+        unpack<BF16, VEC>(cb, y);
+        if (!copied) {
+          if (partners) {
 #pragma unroll
-          for (int i = 0; i < VEC; i += 2) {
-            if (x.d0 + i < p.rotary) {
-              const float2 w = turn[(x.d0 + i) >> 1];
-              const float f = a[i], g = a[i + 1];
-              a[i] = f * w.x - g * w.y;
-              a[i + 1] = g * w.x + f * w.y;
+            for (int e = 0; e < VEC; ++e) {
+              const float f = x[e], g = y[e];
+              x[e] = f * cs[e] - g * sn[e];
+              y[e] = g * cs[e] + f * sn[e];
             }
-            if (x.d1 + i < p.rotary) {
-              const float2 w = turn[(x.d1 + i) >> 1];
-              const float f = b[i], g = b[i + 1];
-              b[i] = f * w.x - g * w.y;
-              b[i + 1] = g * w.x + f * w.y;
+          } else if (p.interleaved) {
+            if constexpr (VEC >= 2) {
+#pragma unroll
+              for (int e = 0; e < VEC / 2; ++e) {
+                const float f = x[2 * e], g = x[2 * e + 1], u = y[2 * e], w = y[2 * e + 1];
+                if (rot0 + 2 * e < p.rotary) {
+                  x[2 * e] = f * cs[e] - g * sn[e];
+                  x[2 * e + 1] = g * cs[e] + f * sn[e];
+                }
+                if (rot1 + 2 * e < p.rotary) {
+                  y[2 * e] = u * cs[VEC / 2 + e] - w * sn[VEC / 2 + e];
+                  y[2 * e + 1] = w * cs[VEC / 2 + e] + u * sn[VEC / 2 + e];
+                }
+              }
             }
           }
         }
+        if (F8 && cached) {
+          const float *scales = copied ? c.value_scale : c.key_scale;
+          const float by = scales ? 1.f / scales[head] : 1.f;
+          if (d0 < c.dim) store_e4m3<VEC, ALIGNED>(dst + d0, x, by);
+          if (d1 < c.dim) store_e4m3<VEC, ALIGNED>(dst + d1, y, by);
+          continue;
+        }
+        ca = pack<BF16, VEC>(x);
+        cb = pack<BF16, VEC>(y);
       }
-      if (F8 && x.cached) {
-        uint8_t *codes = reinterpret_cast<uint8_t *>(x.dst);
-        store_e4m3<VEC, ALIGNED>(codes + x.d0, a, x.scale);
-        if (both) store_e4m3<VEC, ALIGNED>(codes + x.d1, b, x.scale);
-        continue;
-      }
-      ca = pack<BF16, VEC>(a);
-      cb = pack<BF16, VEC>(b);
+      if (d0 < c.dim) store<VEC, ALIGNED>(reinterpret_cast<uint16_t *>(dst) + d0, ca);
+      if (d1 < c.dim) store<VEC, ALIGNED>(reinterpret_cast<uint16_t *>(dst) + d1, cb);
     }
-    store<VEC, ALIGNED>(x.dst + x.d0, ca);
-    if (both) store<VEC, ALIGNED>(x.dst + x.d1, cb);
   }
 }
 
 template <bool BF16, bool F8>
-void launch(const AppendParams &p, int vec, bool aligned, unsigned blocks, cudaStream_t stream) {
-  if (vec == 8) append_kernel<BF16, F8, 8, true><<<blocks, kAppendThreads, 0, stream>>>(p);
-  else if (vec == 4) append_kernel<BF16, F8, 4, true><<<blocks, kAppendThreads, 0, stream>>>(p);
-  else if (vec == 2) append_kernel<BF16, F8, 2, false><<<blocks, kAppendThreads, 0, stream>>>(p);
-  else append_kernel<BF16, F8, 1, false><<<blocks, kAppendThreads, 0, stream>>>(p);
-  GCB_CUDA(cudaGetLastError());
+void launch(const AppendParams &p, int vec, unsigned blocks, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kAppendThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  GCB_CUDA(cudaLaunchKernelEx(&cfg, vec == 8   ? append_kernel<BF16, F8, 8, true>
+                                    : vec == 4 ? append_kernel<BF16, F8, 4, true>
+                                    : vec == 2 ? append_kernel<BF16, F8, 2, false>
+                                               : append_kernel<BF16, F8, 1, false>, p));
   count_launch();
 }
 
@@ -305,12 +305,12 @@ void paged_kv_append(const gcb200_paged_cache &cache, const AppendArgs &a, cudaS
   int64_t all = int64_t(reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) | 2 * (p.k_token | p.k_head | p.v_token | p.v_head);
   if (a.q) all |= int64_t(reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.q_out)) | 2 * (p.q_token | p.q_head | p.o_token | p.o_head);
   const int64_t pieces = a.interleaved ? 0 : (half | rest);
-  int vec = all % 16 == 0 && pieces % 8 == 0 ? 8 : all % 8 == 0 && pieces % 4 == 0 ? 4 : pieces % 2 == 0 ? 2 : 1;
+  const int vec = all % 16 == 0 && pieces % 8 == 0 ? 8 : all % 8 == 0 && pieces % 4 == 0 ? 4 : pieces % 2 == 0 ? 2 : 1;
   const int64_t chunks = cache.head_dim / vec;
   const int64_t rotated_units = a.interleaved || !a.rotary_dim ? 0 : half / vec + (rest / vec + 1) / 2;
   p.units = int(std::max((chunks + 1) / 2, rotated_units));
   const bool bf16 = cache.dtype == GCB200_BF16, f8 = cache.cache_dtype == GCB200_F8_E4M3;
-  (bf16 ? (f8 ? launch<true, true> : launch<true, false>) : (f8 ? launch<false, true> : launch<false, false>))(p, vec, vec >= 4, unsigned(a.tokens), stream);
+  (bf16 ? (f8 ? launch<true, true> : launch<true, false>) : (f8 ? launch<false, true> : launch<false, false>))(p, vec, unsigned(a.tokens), stream);
 }
 
 } // namespace gcb

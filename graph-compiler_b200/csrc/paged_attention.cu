@@ -8,7 +8,7 @@
 //    block adds up the lengths itself and takes an equal share of all tiles of tokens (paged_index.h).  Units (a sequence's KV
 //    head) that a border cuts leave f32 parts in the workspace, which a second kernel, started behind the first by a dependent
 //    launch, joins in the order of the blocks: the same bits every time, and no counter that a call leaves behind.
-//  * A warp fetches its own tokens (16 or 32 of a tile) with asynchronous 16-byte copies, three tiles ahead, and waits for nobody:
+//  * A warp fetches its own tokens (16 or 32 of a tile) with asynchronous 16-byte copies, two or three tiles ahead, and waits for nobody:
 //    page numbers come one tile further ahead, so that no copy waits for the table.  Rows behind the sequence's end are filled with
 //    zeros by the copy.
 //  * Products on the tensor cores with the TOKENS on the instruction's 16-row side and the query heads of the KV head on its
@@ -38,6 +38,13 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kMaxBlocks = 592;   // the workspace has two parts for each
 constexpr float kLazy = 8.f;
 
+// The workspace: a Cut for every block, then two parts for every block.  Part of a cut unit: [cols][dim] f32 sums, then m and l of
+// each column.
+struct Cut {
+  int64_t begin;         // the unit's first tile in the row of all tiles
+  int seq, unit, tiles;  // tiles 0: this border cuts nothing, or not as the first one
+  int per;
+};
 struct PagedAttParams {
   PagedCache c;
   const uint16_t *q;
@@ -45,6 +52,7 @@ struct PagedAttParams {
   int64_t q_seq, q_head, o_seq, o_head;   // elements
   const int32_t *lengths;
   float *lse, *parts;
+  Cut *cuts;
   float scale_log2e;
   int heads, group, sets, window, blocks, least;   // sets: of query heads per KV head, each the columns of one product
   bool q_aligned, same_strides;
@@ -58,17 +66,14 @@ template <bool F8, int DP, int NT> struct Shape {
   static constexpr int kTile = kWarps * kTokens;
   static constexpr int kSlot = 2 * kTokens * kRow;          // a warp's keys and values of one tile
   static constexpr int kCols = 8 * NT;                      // query heads
-#ifdef GCB_ST
-  static constexpr int kStages = GCB_ST;
-#else
-  static constexpr int kStages = F8 && DP >= 128 ? 2 : 3;
-#endif
+  // Three blocks to an SM with 64 KB each, where their registers allow it; else two (one with heads of 256) and three stages.
+  static constexpr int kResident = NT == 1 && DP <= 128 ? 3 : DP <= 128 ? 2 : 1;
+  static constexpr int kStages = kResident == 3 && kSlot == 8192 ? 2 : 3;
   static constexpr int kQRow = DP * 2 + 16;                 // bytes, padded against bank conflicts
   static constexpr int kQ = kCols * kQRow;
   static constexpr int kBytes = kStages * kWarps * kSlot + (kStages + 1) * kQ;
   static_assert(kCols * DP * 4 <= kSlot, "a warp's results fit where its tokens were");
 };
-// Part of a cut unit in the workspace: [cols][dim] f32 sums, then m and l of each column.
 __host__ __device__ __forceinline__ int64_t part_floats(int cols, int dim) { return int64_t(cols) * (dim + 2); }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -159,7 +164,7 @@ template <int CHUNKS> __device__ __forceinline__ uint32_t chunk_at(int r, int ch
 
 // FULL: head_dim is DP, and nothing has to ask where it ends.
 template <bool BF16, bool F8, int DP, int NT, bool FULL>
-__global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_constant__ PagedAttParams p) {
+__global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_attention_kernel(const __grid_constant__ PagedAttParams p) {
   using S = Shape<F8, DP, NT>;
   constexpr bool kMmaBf16 = BF16 && !F8;
   constexpr int kStages = S::kStages, kSteps = DP / 16, kSubs = S::kTokens / 16;
@@ -168,6 +173,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
   __shared__ int64_t pre[kThreads + 1];
   __shared__ Place found;
   __shared__ float stat_m[kWarps][S::kCols], stat_l[kWarps][S::kCols];
+  __shared__ __align__(16) float share[kWarps][kWarps][S::kCols];   // each warp's own copy: what part of the sum the warps' results are
 
   const PagedCache &c = p.c;
   const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x >> 5), 0);   // known to be the same in all lanes
@@ -178,6 +184,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
 
   const int64_t total = count_tiles<S::kTile>(p, units, pre), per = share_of(total, p.blocks, p.least);
   const int64_t begin = int64_t(blockIdx.x) * per, stop = min(total, begin + per);
+  Cut cut{0, 0, 0, 0, 0};
 
   if (begin < stop) {
     Place at = locate<S::kTile>(p, units, pre, begin, &found);
@@ -189,6 +196,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
     Cursor ahead = comp;   // of the tile whose page numbers are being fetched
     const int count = int(stop - begin);
     const int first_tile = comp.tile;
+    if (first_cut(blockIdx.x, per, begin - first_tile, begin - first_tile + comp.tiles)) cut = Cut{begin - first_tile, comp.seq, comp.unit, comp.tiles, int(per)};
 
     uint8_t *mine = smem + warp * kStages * S::kSlot;
     uint8_t *qring = smem + kWarps * kStages * S::kSlot;
@@ -509,41 +517,51 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
         const bool whole = begins && unit_ends;
         float *out_part = p.parts + (2 * int64_t(blockIdx.x) + (begins ? 1 : 0)) * part_floats(S::kCols, dim);
         const float vscale = F8 && c.value_scale ? c.value_scale[kv] : 1.f;
+        // lane (w, h) of each warp: what warp w's result of column h counts
+        float top_m[NT], sum_l[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float mine_m = stat_m[lane >> 3][n * 8 + (lane & 7)];
+          float t = fmaxf(mine_m, __shfl_xor_sync(0xFFFFFFFFu, mine_m, 8));
+          t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 16));
+          const float part = ex2(mine_m - finite_ref(t));
+          float sum = stat_l[lane >> 3][n * 8 + (lane & 7)] * part;
+          sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 8);
+          sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
+          top_m[n] = t;
+          sum_l[n] = sum;
+          share[warp][lane >> 3][n * 8 + (lane & 7)] = whole ? part / sum * vscale : part;
+        }
+        __syncwarp();
         for (int i = threadIdx.x; i < NT * dim; i += kThreads) {
-          const int n = i / dim, d = i - n * dim;
+          const int n = NT == 1 ? 0 : i / dim, d = i - n * dim;
           float sum[8] = {};
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) {
             const float4 *src = reinterpret_cast<const float4 *>(smem + (w * kStages + stage) * S::kSlot) + (d * S::kCols + n * 8) / 4;
-            const float4 a = src[0], b = src[1];
-            const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int h = 0; h < 8; ++h) {
-              float top_m = stat_m[0][n * 8 + h];
-#pragma unroll
-              for (int w2 = 1; w2 < kWarps; ++w2) top_m = fmaxf(top_m, stat_m[w2][n * 8 + h]);
-              sum[h] = fmaf(v[h], ex2(stat_m[w][n * 8 + h] - finite_ref(top_m)), sum[h]);
-            }
+            const float4 *by = reinterpret_cast<const float4 *>(&share[warp][w][n * 8]);
+            const float4 a = src[0], b = src[1], x0 = by[0], x1 = by[1];
+            sum[0] = fmaf(a.x, x0.x, sum[0]); sum[1] = fmaf(a.y, x0.y, sum[1]); sum[2] = fmaf(a.z, x0.z, sum[2]); sum[3] = fmaf(a.w, x0.w, sum[3]);
+            sum[4] = fmaf(b.x, x1.x, sum[4]); sum[5] = fmaf(b.y, x1.y, sum[5]); sum[6] = fmaf(b.z, x1.z, sum[6]); sum[7] = fmaf(b.w, x1.w, sum[7]);
           }
+          const int head = kv * p.group + set * S::kCols + n * 8;
 #pragma unroll
           for (int h = 0; h < 8; ++h) {
-            const int col = n * 8 + h;
+            if (n * 8 + h >= cols) break;
+            if (whole) p.out[comp.seq * p.o_seq + (head + h) * p.o_head + d] = f32_to_half<BF16>(sum[h]);
+            else out_part[int64_t(n * 8 + h) * dim + d] = sum[h];
+          }
+        }
+        if (warp == 0 && lane < 8) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const int col = n * 8 + lane, head = kv * p.group + set * S::kCols + col;
             if (col >= cols) break;
-            float top_m = stat_m[0][col], sum_l = 0.f;
-#pragma unroll
-            for (int w2 = 1; w2 < kWarps; ++w2) top_m = fmaxf(top_m, stat_m[w2][col]);
-#pragma unroll
-            for (int w2 = 0; w2 < kWarps; ++w2) sum_l = fmaf(stat_l[w2][col], ex2(stat_m[w2][col] - finite_ref(top_m)), sum_l);
-            const int head = kv * p.group + set * S::kCols + col;
-            if (whole) {
-              p.out[comp.seq * p.o_seq + head * p.o_head + d] = f32_to_half<BF16>(sum[h] / sum_l * vscale);
-              if (d == 0 && p.lse) p.lse[int64_t(comp.seq) * p.heads + head] = (finite_ref(top_m) + log2f(sum_l)) * 0.6931471805599453f;
-            } else {
-              out_part[int64_t(col) * dim + d] = sum[h];
-              if (d == 0) {
-                out_part[int64_t(S::kCols) * dim + 2 * col] = top_m;
-                out_part[int64_t(S::kCols) * dim + 2 * col + 1] = sum_l;
-              }
+            if (!whole) {
+              out_part[int64_t(S::kCols) * dim + 2 * col] = top_m[n];
+              out_part[int64_t(S::kCols) * dim + 2 * col + 1] = sum_l[n];
+            } else if (p.lse) {
+              p.lse[int64_t(comp.seq) * p.heads + head] = (finite_ref(top_m[n]) + log2f(sum_l[n])) * 0.6931471805599453f;
             }
           }
         }
@@ -560,6 +578,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
     cp_async_wait<0>();
   }
 
+  if (threadIdx.x == 0) p.cuts[blockIdx.x] = cut;
   // ---- sequences of which nothing is seen
   for (int s = blockIdx.x; s < c.table.sequences; s += gridDim.x) {
     const Seen see = seen_of(c.table, p.lengths[s], p.window);
@@ -574,52 +593,67 @@ __global__ void __launch_bounds__(kThreads) paged_attention_kernel(const __grid_
   }
 }
 
-// Block (i - 1, y): the unit that border i cuts first, columns y, y + gridDim.y, ...
-template <bool BF16, bool F8, int DP, int NT>
+// Block (i - 1, y): the unit that border i cuts first; warp w of it column 4 y + w.  The lanes weigh 32 parts at a time by their
+// maxima, then add the parts up, four elements to a lane and eight parts under way.
+template <bool BF16, bool F8, int NT>
 __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_constant__ PagedAttParams p) {
-  using S = Shape<F8, DP, NT>;
-  __shared__ int64_t pre[kThreads + 1];
-  __shared__ Place found;
+  constexpr int kCols = 8 * NT;
   const PagedCache &c = p.c;
-  const int units = c.kv_heads * p.sets, dim = c.dim;
-  const int64_t i = int64_t(blockIdx.x) + 1;
-  // The lengths may be read before the wait: the kernel ahead let this one start behind its own wait for everything before it.
-  const int64_t total = count_tiles<S::kTile>(p, units, pre), per = share_of(total, p.blocks, p.least);
-  bool cut = i * per < total;
-  Place at{};
-  int64_t begin = 0, end = 0;
-  int unit = 0;
-  if (cut) {
-    at = locate<S::kTile>(p, units, pre, i * per, &found);
-    const int tiles = tiles_of(seen_of(c.table, p.lengths[at.seq], p.window), S::kTile);
-    unit = min(units - 1, int(at.rest / max(1, tiles)));
-    begin = i * per - (at.rest - int64_t(unit) * tiles);
-    end = begin + tiles;
-    cut = first_cut(i, per, begin, end);
-  }
+  const int lane = threadIdx.x & 31, col = int(blockIdx.y) * kWarps + int(threadIdx.x >> 5), dim = c.dim;
   pdl_wait();
   pdl_launch_dependents();
-  if (!cut) return;
-  const int kv = unit / p.sets, set = unit - kv * p.sets, cols = min(S::kCols, p.group - set * S::kCols);
-  const int64_t b0 = begin / per, b1 = (end - 1) / per, floats = part_floats(S::kCols, dim);
-  const float vscale = F8 && c.value_scale ? c.value_scale[kv] : 1.f;
-  for (int col = blockIdx.y; col < cols; col += gridDim.y) {
-    float m = -INFINITY;
-    for (int64_t b = b0; b <= b1; ++b) m = fmaxf(m, p.parts[part_slot(b, per, begin) * floats + int64_t(S::kCols) * dim + 2 * col]);
-    const float ref = finite_ref(m);
-    const int head = kv * p.group + set * S::kCols + col;
-    for (int d = threadIdx.x; d < dim; d += kThreads) {
-      float l = 0.f, sum = 0.f;
-      for (int64_t b = b0; b <= b1; ++b) {
-        const float *part = p.parts + part_slot(b, per, begin) * floats;
-        const float w = ex2(part[int64_t(S::kCols) * dim + 2 * col] - ref);
-        l = fmaf(part[int64_t(S::kCols) * dim + 2 * col + 1], w, l);
-        sum = fmaf(part[int64_t(col) * dim + d], w, sum);
-      }
-      p.out[at.seq * p.o_seq + head * p.o_head + d] = f32_to_half<BF16>(sum / l * vscale);
-      if (d == 0 && p.lse) p.lse[int64_t(at.seq) * p.heads + head] = (ref + log2f(l)) * 0.6931471805599453f;
+  const Cut cut = p.cuts[blockIdx.x + 1];
+  if (cut.tiles == 0) return;
+  const int kv = cut.unit / p.sets, set = cut.unit - kv * p.sets;
+  if (col >= min(kCols, p.group - set * kCols)) return;
+  const int b0 = int(cut.begin / cut.per), count = int((cut.begin + cut.tiles - 1) / cut.per) - b0 + 1;
+  const int64_t floats = part_floats(kCols, dim);
+  // part i of the unit: the first block's second place if the unit begins there, every other block's first
+  const float *first = p.parts + part_slot(b0, cut.per, cut.begin) * floats, *rest = p.parts + 2 * int64_t(b0) * floats;
+  auto part = [&](int i) { return i == 0 ? first : rest + 2 * int64_t(i) * floats; };
+  float m = -INFINITY;
+  for (int i = lane; i < count; i += 32) m = fmaxf(m, part(i)[int64_t(kCols) * dim + 2 * col]);
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, i));
+  const float ref = finite_ref(m);
+  float l = 0.f;
+  float4 sum[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  for (int i0 = 0; i0 < count; i0 += 32) {
+    float w = 0.f;
+    if (i0 + lane < count) {
+      const float2 ml = *reinterpret_cast<const float2 *>(part(i0 + lane) + int64_t(kCols) * dim + 2 * col);
+      w = ex2(ml.x - ref);
+      l = fmaf(ml.y, w, l);
+    }
+    const int n = min(32, count - i0);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float by = __shfl_sync(0xFFFFFFFFu, w, i);
+      const float *from = part(i0 + i) + int64_t(col) * dim;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (h * 128 + lane * 4 < dim) {
+          const float4 v = *reinterpret_cast<const float4 *>(from + h * 128 + lane * 4);
+          sum[h].x = fmaf(v.x, by, sum[h].x);
+          sum[h].y = fmaf(v.y, by, sum[h].y);
+          sum[h].z = fmaf(v.z, by, sum[h].z);
+          sum[h].w = fmaf(v.w, by, sum[h].w);
+        }
     }
   }
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, i);
+  const float scale = (F8 && c.value_scale ? c.value_scale[kv] : 1.f) / l;
+  const int head = kv * p.group + set * kCols + col;
+  uint16_t *out = p.out + cut.seq * p.o_seq + head * p.o_head;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if (h * 128 + lane * 4 < dim) {
+      const float v[4] = {sum[h].x, sum[h].y, sum[h].z, sum[h].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[h * 128 + lane * 4 + e] = f32_to_half<BF16>(v[e] * scale);
+    }
+  if (lane == 0 && p.lse) p.lse[int64_t(cut.seq) * p.heads + head] = (ref + log2f(l)) * 0.6931471805599453f;
 }
 
 void require(bool ok, const char *what) {
@@ -659,7 +693,7 @@ template <bool BF16, bool F8, int DP, int NT, bool FULL> void launch(PagedAttPar
   p.blocks = std::min(kMaxBlocks, dev.sm_count * r);
   p.least = 1;
   launch_dependent(kernel, dim3(unsigned(p.blocks)), S::kBytes, stream, p);
-  if (p.blocks > 1) launch_dependent(paged_join_kernel<BF16, F8, DP, NT>, dim3(unsigned(p.blocks - 1), 4), 0, stream, p);
+  if (p.blocks > 1) launch_dependent(paged_join_kernel<BF16, F8, NT>, dim3(unsigned(p.blocks - 1), 2 * NT), 0, stream, p);
 }
 
 template <bool BF16, bool F8> void launch(const PagedAttParams &p, int cols, DeviceState &dev, cudaStream_t stream) {
@@ -677,7 +711,7 @@ template <bool BF16, bool F8> void launch(const PagedAttParams &p, int cols, Dev
 size_t paged_attention_workspace(int64_t heads, int64_t kv_heads, int64_t head_dim) {
   require(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads < 65536, "paged attention: heads must be a multiple of kv_heads");
   require(head_dim > 0 && head_dim <= 256, "paged attention: head_dim must be at most 256");
-  return size_t(2) * kMaxBlocks * size_t(part_floats(columns(heads / kv_heads, head_dim), int(head_dim))) * sizeof(float);
+  return kMaxBlocks * (sizeof(Cut) + 2 * size_t(part_floats(columns(heads / kv_heads, head_dim), int(head_dim))) * sizeof(float));
 }
 
 void paged_attention(const gcb200_paged_cache &cache, const PagedAttentionArgs &a, cudaStream_t stream) {
@@ -700,7 +734,9 @@ void paged_attention(const gcb200_paged_cache &cache, const PagedAttentionArgs &
   p.same_strides = p.c.key_page == p.c.value_page && p.c.key_token == p.c.value_token;
   p.lengths = a.lengths;
   p.lse = a.lse;
-  p.parts = static_cast<float *>(a.workspace);
+  static_assert(kMaxBlocks * sizeof(Cut) % 16 == 0, "the parts are read in fours");
+  p.cuts = static_cast<Cut *>(a.workspace);
+  p.parts = reinterpret_cast<float *>(p.cuts + kMaxBlocks);
   p.scale_log2e = a.scale * 1.4426950408889634f;
   p.heads = int(a.heads);
   p.group = int(a.heads / cache.kv_heads);
