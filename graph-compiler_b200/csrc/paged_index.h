@@ -46,8 +46,12 @@ GCB_HD Seen seen_of(const PageTable &t, int length, int window) {
 // inside, are one row of `total` that is cut into equal parts: block i takes [i per, (i + 1) per).  A unit may be cut by the borders
 // of several blocks; each then keeps a part of its softmax, and the parts are joined in the order of the blocks.
 GCB_HD int tiles_of(const Seen &s, int tile) { return (s.end - s.first + tile - 1) / tile; }
+// Large shares are rounded up to fours (never by more than an eighth): where units have 2^n tiles, odd shares leave the blocks at as
+// many different places of a sequence at a time, and 16 sequences x 32 heads x 2048 tokens, 37 tiles to a block, took 104 us instead
+// of 90 with 38 or 40.
 GCB_HD int64_t share_of(int64_t total, int blocks, int least) {
-  const int64_t per = (total + blocks - 1) / blocks;
+  int64_t per = (total + blocks - 1) / blocks;
+  if (per >= 32) per = (per + 3) / 4 * 4;
   return per < least ? least : per;
 }
 // A block keeps at most two parts: of the unit that it continues (0) and of one that it begins and does not end (1).
