@@ -6,7 +6,9 @@
 // f64 in whole turns, reduced by the whole turns there, and only the remaining fraction becomes f32 for sincospi.  All heads of
 // a token share its angles: a block computes them once, into shared memory.
 //
-// Bound by HBM: q read and written, k and v read, the cache's rows written.
+// Bound by HBM: q read and written, k and v read, the cache's rows written.  Small blocks and few rows under way in a thread leave
+// registers for many threads: 8192 tokens of 32 + 2 x 8 heads of 128 (201 MB) 39 us, 5.1 TB/s, with 64 threads and two rows; four
+// rows 42, 128 threads and two rows 41, 128 and four 45.
 #include "decode_ops.h"
 
 #include <algorithm>
@@ -20,7 +22,8 @@ namespace gcb {
 
 namespace {
 
-constexpr int kAppendThreads = 128;
+// Threads of a block: at least the pieces of a row (at most 128 of single elements, 64 of two).
+template <int VEC> constexpr int kAppendThreads = VEC == 1 ? 128 : 64;
 constexpr int kMaxDim = 256;
 
 struct AppendParams {
@@ -92,10 +95,11 @@ template <int VEC, bool ALIGNED> __device__ __forceinline__ void store_e4m3(uint
 }
 
 // One block per token.  A thread has the same piece of every row it takes - two chunks of VEC elements, the partners of a rotation by
-// halves or neighbours - so that it loads its cosines and sines once; it takes rows kBatch at a time and asks for all of them, the
-// first ones before the angles are there.
+// halves or neighbours - so that it loads its cosines and sines once; it asks for kBatch rows at a time, the first ones before
+// the angles are there.
 template <bool BF16, bool F8, int VEC, bool ALIGNED>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads<VEC>) append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int kThreads = kAppendThreads<VEC>;
   __shared__ float2 turn[kMaxDim / 2];   // (cos, sin) of each pair
   pdl_wait();
   pdl_launch_dependents();
@@ -105,13 +109,13 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
   if (seq < 0 || pos < 0) return;   // padding
 
   const int half = p.rotary >> 1, q_rows = p.q ? p.heads : 0, rows = q_rows + 2 * c.kv_heads;
-  const int row_step = kAppendThreads / p.units, row0 = int(threadIdx.x) / p.units, piece = int(threadIdx.x) - row0 * p.units;
+  const int row_step = kThreads / p.units, row0 = int(threadIdx.x) / p.units, piece = int(threadIdx.x) - row0 * p.units;
   // Where the piece lies in a rotated row and in a row that is only copied.
   const bool halves = p.rotary > 0 && !p.interleaved, partners = halves && piece * VEC < half;
   const int rot0 = partners ? piece * VEC : halves ? p.rotary + 2 * (piece - half / VEC) * VEC : 2 * piece * VEC, rot1 = rot0 + (partners ? half : VEC);
   const int copy0 = 2 * piece * VEC, copy1 = copy0 + VEC;
 
-  constexpr int kBatch = 4;
+  constexpr int kBatch = 2;
   Chunk<VEC> a[kBatch], b[kBatch];
   auto fetch = [&](int first) {
 #pragma unroll
@@ -129,7 +133,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     }
   };
   fetch(row0);
-  for (int i = threadIdx.x; i < half; i += kAppendThreads) {
+  for (int i = threadIdx.x; i < half; i += kThreads) {
     const double turns = double(pos) * p.inv_freq[i] * 0.15915494309189533577;   // 1 / (2 pi)
     float s, co;
     sincospif(2.f * float(turns - rint(turns)), &s, &co);
@@ -211,7 +215,7 @@ template <bool BF16, bool F8>
 void launch(const AppendParams &p, int vec, unsigned blocks, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(kAppendThreads);
+  cfg.blockDim = dim3(unsigned(vec == 1 ? kAppendThreads<1> : kAppendThreads<8>));
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
