@@ -325,19 +325,24 @@ __global__ void __launch_bounds__(kW4Threads, 1) matmul_w4_kernel(const __grid_c
           if (row[b] >= rows) break;
           uint4 u = held[b];
           const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-          float down = 1.f, factor = 1.f;
+          float lift = 1.f, down = 1.f, factor = 1.f;
           if constexpr (BF16) {
             // magnitudes compare like their bits; the largest of the k block lies in [2^(e + 14), 2^(e + 15))
             uint32_t big2 = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu), __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
 #pragma unroll
             for (int d = 1; d < 16; d <<= 1) big2 = __vmaxu2(big2, __shfl_xor_sync(0xFFFFFFFFu, big2, d));
-            const int field = int(max(big2 & 0xFFFFu, big2 >> 16) >> 7), e = field == 255 ? 0 : max(field - 127 - 14, -110);
-            down = __uint_as_float(uint32_t(127 - e) << 23);
-            factor = __uint_as_float(uint32_t(127 + e) << 23);
+            const int field = int(max(big2 & 0xFFFFu, big2 >> 16) >> 7), e = field == 255 ? 0 : max(field, 1) - 127 - 14;
+            const int first = e < -100 ? 60 : 0;   // a scale beyond f32's range in two steps
+            lift = __uint_as_float(uint32_t(127 + first) << 23);
+            down = __uint_as_float(uint32_t(127 - e - first) << 23);
+            factor = __uint_as_float(e >= -126 ? uint32_t(127 + e) << 23 : 1u << (149 + e));
           }
           float v[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = half_to_f32<BF16>((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu) * down;
+          for (int e = 0; e < 8; ++e) {
+            v[e] = half_to_f32<BF16>((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu);
+            if (BF16) v[e] = v[e] * lift * down;
+          }
           float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
           if constexpr (BF16) u = make_uint4(pack_half2<false>(v[0], v[1]), pack_half2<false>(v[2], v[3]), pack_half2<false>(v[4], v[5]), pack_half2<false>(v[6], v[7]));
 #pragma unroll
@@ -403,7 +408,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) matmul_w4_kernel(const __grid_c
 #pragma unroll
         for (int g = 0; g < GPB; ++g) {
           float sum[RT][NT][4];
-          // in units of the codes:  acc += scale factor (sum x code - zero sum x);  the second term is what the products start from
+          // acc += scale factor (sum x code - zero sum x);  the second term is what the products start from
           float2 xs[NT][2];   // columns 2 c and 2 c + 1
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
@@ -446,11 +451,11 @@ __global__ void __launch_bounds__(kW4Threads, 1) matmul_w4_kernel(const __grid_c
           for (int t = 0; t < RT; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float s = half_to_f32<BF16>((scale[t][h][g / 2] >> (16 * (g & 1))) & 0xFFFFu);
+              const float s = half_to_f32<BF16>((scale[t][h][g / 2] >> (16 * (g & 1))) & 0xFFFFu) * (h ? 0.0625f / kUnit : 1.f / kUnit);
 #pragma unroll
               for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) acc[t][n][2 * h + i] = fmaf(BF16 ? sum[t][n][2 * h + i] * xs[n][i].x : sum[t][n][2 * h + i], s, acc[t][n][2 * h + i]);
+                for (int i = 0; i < 2; ++i) acc[t][n][2 * h + i] = BF16 ? fmaf(sum[t][n][2 * h + i] * s, xs[n][i].x, acc[t][n][2 * h + i]) : fmaf(sum[t][n][2 * h + i], s, acc[t][n][2 * h + i]);
             }
         }
 #pragma unroll
@@ -465,7 +470,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) matmul_w4_kernel(const __grid_c
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) own[(n * 8 + (i & 1)) * kMeetRow + t * 16 + 8 * (i >> 1)] = acc[t][n][i] * (i >> 1 ? 0.0625f / kUnit : 1.f / kUnit);
+          for (int i = 0; i < 4; ++i) own[(n * 8 + (i & 1)) * kMeetRow + t * 16 + 8 * (i >> 1)] = acc[t][n][i];
       __syncwarp();
       if (lane == 0) mbar_arrive(meet_full);
       meet_parity ^= 1u;

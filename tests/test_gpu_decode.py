@@ -334,6 +334,90 @@ def test_attention_and_append_in_captured_graphs():
     assert lib.device_error() == 0
 
 
+def test_attention_keys_and_values_laid_out_differently():
+    """Keys with heads outside tokens, values with tokens outside heads, and another distance between pages."""
+    g = torch.Generator().manual_seed(12)
+    lengths, kv, D, H = [200, 0, 33, 1], 2, 128, 8
+    for page in (16, 24):
+        table, pages = _table(g, lengths, page)
+        for kk, kind in (("bf16", "bf16"), ("bf16", "e4m3")):
+            keys = _cache(g, pages, kv, page, D, kind, "heads")
+            values = _cache(g, 2 * pages, kv, page, D, kind, "tokens")[::2]
+            ks = vs = torch.full((kv,), 0.03, device="cuda") if kind == "e4m3" else None
+            q = torch.randn(4, H, D, generator=g).bfloat16().cuda()
+            lens = torch.tensor(lengths, dtype=torch.int32).cuda()
+            out = lib.paged_attention(q, keys, values, table.cuda(), lens, 0.08, key_scale=ks, value_scale=vs)
+            want, mag, _ = _attend_want(q, keys, values, table, lengths, 0.08, 0, page, ks, vs)
+            _close(out, want, U["bf16"] * want.abs() + (U["f16" if kind == "e4m3" else "bf16"] + 2.0 ** -13) * mag + 1e-7)
+
+
+def test_attention_negative_lengths_and_scales():
+    g = torch.Generator().manual_seed(13)
+    lengths, page, D = [90, 17], 16, 64
+    table, pages = _table(g, lengths, page)
+    for kind in ("bf16", "e4m3"):
+        keys, values = _cache(g, pages, 1, page, D, kind, "heads"), _cache(g, pages, 1, page, D, kind, "heads")
+        ks = vs = torch.full((1,), 0.03, device="cuda") if kind == "e4m3" else None
+        q = torch.randn(2, 3, D, generator=g).bfloat16().cuda()
+        lse = torch.zeros(2, 3, device="cuda")
+        out = lib.paged_attention(q, keys, values, table.cuda(), torch.tensor([90, -5], dtype=torch.int32).cuda(), -0.2, key_scale=ks, value_scale=vs, lse=lse)
+        want, mag, wl = _attend_want(q, keys, values, table, [90, 0], -0.2, 0, page, ks, vs)
+        _close(out, want, U["bf16"] * want.abs() + (U["f16" if kind == "e4m3" else "bf16"] + 2.0 ** -13) * mag + 1e-7)
+        assert (lse[1] == -math.inf).all() and not _raw(out[1]).any()
+        flat = lib.paged_attention(q, keys, values, table.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(), 0.0, key_scale=ks, value_scale=vs)
+        want, mag, _ = _attend_want(q, keys, values, table, lengths, 0.0, 0, page, ks, vs)      # the mean of the values
+        _close(flat, want, U["bf16"] * want.abs() + (U["f16" if kind == "e4m3" else "bf16"] + 2.0 ** -13) * mag + 1e-7)
+
+
+@pytest.mark.parametrize("kind", ["f16", "e4m3"])
+def test_attention_one_large_share_and_a_long_tail(kind):
+    """One token takes half of the softmax, thousands of others below 2^-12 of it the other half: none of them may vanish.  Their
+    exponentials are far below f16's smallest normal number."""
+    S, D, page = 20000, 64, 32
+    table = torch.arange(S // page, dtype=torch.int32)[None].cuda()
+    keys = torch.zeros(S // page, 1, page, D).to(T[kind]).cuda()
+    values = torch.ones(S // page, 1, page, D).to(T[kind]).cuda()
+    keys[3, 0, 5, 0] = 1.0
+    values[3, 0, 5] = -1.0
+    q = torch.zeros(1, 1, D, dtype=torch.float16)
+    q[0, 0, 0] = 10.0
+    q = q.cuda()
+    one = torch.ones(1, device="cuda") if kind == "e4m3" else None
+    out = lib.paged_attention(q, keys, values, table, torch.tensor([S], dtype=torch.int32).cuda(), 1.0, key_scale=one, value_scale=one)
+    w = math.exp(10.0)
+    want = torch.full((1, 1, D), (S - 1 - w) / (S - 1 + w), dtype=torch.float64)
+    _close(out, want, U["f16"] * want.abs() + (U["f16"] + 2.0 ** -13))
+    q[0, 0, 0] = 18.0           # the others: e^-18, below 2^-25
+    keys[3, 0, 5, 0] = 1.0
+    out = lib.paged_attention(q, keys, values, table, torch.tensor([S], dtype=torch.int32).cuda(), 1.0, key_scale=one, value_scale=one)
+    w = math.exp(18.0)
+    want = torch.full((1, 1, D), (S - 1 - w) / (S - 1 + w), dtype=torch.float64)
+    _close(out, want, U["f16"] * want.abs() + (U["f16"] + 2.0 ** -13))
+
+
+def test_first_use_of_a_variant_inside_a_capture():
+    """A kernel variant that no call has used yet, captured and replayed."""
+    g = torch.Generator().manual_seed(14)
+    lengths, page, D = [300, 77], 16, 96
+    table, pages = _table(g, lengths, page)
+    keys, values = _cache(g, pages, 1, page, D, "f16", "heads"), _cache(g, pages, 1, page, D, "f16", "heads")
+    q = torch.randn(2, 13, D, generator=g).half().cuda()
+    lens, tab = torch.tensor(lengths, dtype=torch.int32).cuda(), table.cuda()
+    codes, scales = torch.randint(0, 256, (48, 300), generator=g, dtype=torch.uint8).cuda(), torch.rand(48, 10, generator=g).half().cuda()
+    w = lib.pack_w4(codes, scales, 600, 64, zeros=torch.randint(0, 16, (48, 10), generator=g, dtype=torch.uint8).cuda())
+    x = torch.randn(11, 600, generator=g).half().cuda()
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = lib.paged_attention(q, keys, values, tab, lens, 0.1)
+        y = lib.matmul_w4(x, w)
+    gr.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, lib.paged_attention(q, keys, values, tab, lens, 0.1)) and torch.equal(y, lib.matmul_w4(x, w))
+    want, mag, _ = _attend_want(q, keys, values, table, lengths, 0.1, 0, page, None, None)
+    _close(out, want, U["f16"] * want.abs() + (U["f16"] + 2.0 ** -13) * mag + 1e-7)
+
+
 # ----------------------------------------------------------------------------- append
 def _rotated(x, pos, inv, interleaved):
     """(rotated, |a| + |b| of each element's pair) in 64 bits."""
@@ -580,6 +664,38 @@ def test_w4_same_bits_every_time_and_rows_alone():
             z = lib.matmul_w4(x, p)
         other.synchronize()
         assert torch.equal(z, y)
+
+
+def test_w4_long_rows_and_what_does_not_fit():
+    """Rows of x that only a cluster's shared memory holds, fewer rows at a time where sixteen do not fit, and too long ones."""
+    _w4_check(1, 40, 60000, 128, False, False, False, "bf16")
+    _w4_check(16, 24, 30001, 64, True, True, False, "f16")
+    _w4_check(3, 33, 100000, 256, False, False, False, "bf16")
+    codes, scales = torch.zeros(16, 130000, dtype=torch.uint8, device="cuda"), torch.ones(16, 1, dtype=torch.bfloat16, device="cuda")
+    p = lib.pack_w4(codes, scales, 260000, 260096)
+    with pytest.raises(lib.GcB200Error, match="does not fit"):
+        lib.matmul_w4(torch.zeros(1, 260000, dtype=torch.bfloat16, device="cuda"), p)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_w4_rows_of_unequal_magnitude(dtype):
+    """Rows, and the k blocks of a row, whose magnitudes lie far apart, subnormal ones and zeros among them."""
+    g = torch.Generator().manual_seed(3)
+    M, N, K = 12, 64, 768
+    codes, scales = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8), (0.5 + torch.rand(N, K // 128, generator=g)).to(T[dtype])
+    w = (torch.stack([codes & 15, codes >> 4], -1).flatten(1).double() - 8) * scales.double().repeat_interleave(128, 1)
+    e = torch.randint(-30, 31, (M, K // 128), generator=g) if dtype == "bf16" else torch.randint(-9, 9, (M, K // 128), generator=g)
+    x = torch.randn(M, K, generator=g) * (2.0 ** e).repeat_interleave(128, 1)
+    x[0] = 0
+    x[1] = 1e-40 if dtype == "bf16" else 6e-8
+    x[2, :128] = 3e38 if dtype == "bf16" else 6e4
+    x[2, 128:] = 0
+    x = x.to(T[dtype])
+    y = lib.matmul_w4(x.cuda(), lib.pack_w4(codes.cuda(), scales.cuda(), K, 128))
+    want, mag = x.double() @ w.T, x.double().abs() @ w.abs().T
+    top = 3.39e38 if dtype == "bf16" else 65504.0
+    ok = mag < top / 2          # what is larger may overflow the result's type, or the f32 sum
+    _close(y.cpu().double()[ok], want[ok], (U[dtype] * want.abs() + 2.0 ** -14 * mag + torch.finfo(T[dtype]).smallest_normal * U[dtype] * 2)[ok])
 
 
 # ----------------------------------------------------------------------------- refusals, and the operators as a run
