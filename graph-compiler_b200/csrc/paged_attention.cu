@@ -376,8 +376,9 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 if (!FULL && (j + h) * 16 >= dim) break;   // an odd number of chunks: nobody has filled the last one
-                const uint32_t a[4] = {e4m3x2_to_f16x2(r[2 * h] & 0xFFFFu), e4m3x2_to_f16x2(r[2 * h + 1] & 0xFFFFu), e4m3x2_to_f16x2(r[2 * h] >> 16),
-                                       e4m3x2_to_f16x2(r[2 * h + 1] >> 16)};
+                uint32_t a[4];
+                e4m3x4_to_f16x2(r[2 * h], a[0], a[2]);
+                e4m3x4_to_f16x2(r[2 * h + 1], a[1], a[3]);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) mma_16816<kMmaBf16>(h ? sd[u][n] : sc[u][n], a, qf[j + h][n][0], qf[j + h][n][1]);
               }
@@ -468,7 +469,9 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
               for (int h = 0; h < 2; ++h) {
                 if (!FULL && (j + h) * 16 >= dim) break;
                 const uint32_t t0 = __byte_perm(r[h], 0, 0x3120), t1 = __byte_perm(r[h + 2], 0, 0x3120);
-                const uint32_t a[4] = {e4m3x2_to_f16x2(t0 & 0xFFFFu), e4m3x2_to_f16x2(t0 >> 16), e4m3x2_to_f16x2(t1 & 0xFFFFu), e4m3x2_to_f16x2(t1 >> 16)};
+                uint32_t a[4];
+                e4m3x4_to_f16x2(t0, a[0], a[1]);
+                e4m3x4_to_f16x2(t1, a[2], a[3]);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) mma_16816<kMmaBf16>(acc[j + h][n], a, pt[n][0], pt[n][1]);
               }

@@ -206,7 +206,8 @@ int gcb200_attention_bf16(const void *Q, const void *K, const void *V, void *O, 
  * caches' base addresses and strides are multiples of 16 bytes.  cache_dtype is dtype, or GCB200_F8_E4M3: a cached number is
  * then code * scale of its KV head.  A page number outside [0, pages) that a call meets is never followed: the call records
  * code 9 in the device error word (gcb200_device_error), and those tokens count as zeros (attention) or are not written
- * (append). */
+ * (append).  Calls may be captured into a graph, once any call of this library has run on the device; a replay follows the page
+ * table, positions and lengths that device memory holds then. */
 typedef enum { GCB200_F16 = 1, GCB200_BF16 = 2, GCB200_F8_E4M3 = 10 } gcb200_dtype; /* dnnl_data_type_t's codes where it has one */
 typedef struct {
   int dtype;                      /* queries, new keys and values, results: GCB200_BF16 or GCB200_F16 */
@@ -254,7 +255,7 @@ int gcb200_paged_attention(const gcb200_paged_cache *cache, const void *q, const
  * group is 32, 64 or a multiple of 128.  gcb200_w4_pack lays the weights out once, in the order in which the kernel reads them:
  * codes [N] rows of (K + 1) / 2 bytes (even k in the low half of a byte), scales and zeros [N][ceil(K / group)] (zeros NULL: 8);
  * row strides are in elements.  packed: gcb200_w4_packed_bytes() bytes, 16-byte aligned.  The scales' type is that of the X the
- * weights will meet.  Any M; more than 16 rows read the weights once for every 16.  NaN or an infinity in a row of X makes that
+ * weights will meet.  Y may not overlap X.  Any M; more than 16 rows read the weights once for every 16.  NaN or an infinity in a row of X makes that
  * row's results NaN, and no other's. */
 int gcb200_w4_packed_bytes(int64_t N, int64_t K, int64_t group, int has_zeros, size_t *bytes);
 int gcb200_w4_pack(const uint8_t *codes, int64_t codes_stride, const void *scales, int64_t scales_stride, const uint8_t *zeros,

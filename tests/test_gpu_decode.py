@@ -162,6 +162,20 @@ def test_attention_many_sequences():
     _attend_check("f16", "e4m3", [int(x) for x in r.randint(0, 20, 700)], 2, 1, 64, 16)
 
 
+def test_attention_more_sequences_than_a_grid_has_rows():
+    """Seventy thousand sequences of one token, every seventh empty: each gives its own value row, bit for bit."""
+    S, D = 70000, 16
+    g = torch.Generator(device="cuda").manual_seed(0)
+    keys, values = (torch.randn(S, 1, 1, D, generator=g, device="cuda").bfloat16() for _ in range(2))
+    table = torch.randperm(S, generator=g, device="cuda").to(torch.int32)[:, None]
+    lens = (torch.arange(S, device="cuda") % 7 != 0).to(torch.int32)
+    q = torch.randn(S, 2, D, generator=g, device="cuda").bfloat16()
+    out = lib.paged_attention(q, keys, values, table, lens, 1.0)
+    want = torch.where((lens > 0)[:, None, None], values[table[:, 0].long(), :, 0], torch.zeros_like(q[:, :1])).expand(-1, 2, -1)
+    assert torch.equal(out, want)
+    assert lib.device_error() == 0
+
+
 def test_attention_large_scores():
     """Scores in the hundreds: one token takes nearly everything, and maxima grow along the sequence."""
     # f32 scores of this size are off by up to 2^9 2^-20 instead of 2^6 2^-20: the case keeps the tolerance by having exact scores
