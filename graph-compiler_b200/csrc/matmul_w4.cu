@@ -50,31 +50,45 @@ struct W4PackParams {
   int gpb, bytes;
 };
 
-// One block of 256 threads packs one 16 x 128 block; a thread one 32-bit word.  Word w of a lane in half h covers
+// 64 threads pack one 16 x 128 block, a thread 16 bytes: the four words of a lane in one half.  Word w of a lane in half h covers
 // k = 64 h + 32 (w >> 1) + 8 c + 4 (w & 1) + {0, 1, 2, 3} of outputs r and r + 8 (r = lane / 4, c = lane % 4): the registers
 // s = 0..3 of the instruction's A operand, each a pair of k in the word's halves.  Within a half, code s lies where a mask finds
 // it: at bit 2, at bit 6, and, with the half's bytes exchanged, at bit 2 and bit 6 again.
-__global__ void __launch_bounds__(256) w4_pack_kernel(const __grid_constant__ W4PackParams p) {
+constexpr int kPackBlocks = 4;   // k blocks of a thread block: 256 contiguous bytes of each row of codes
+__global__ void __launch_bounds__(kPackBlocks * 64) w4_pack_kernel(const __grid_constant__ W4PackParams p) {
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t kb = blockIdx.x, nt = blockIdx.y + int64_t(blockIdx.z) * gridDim.y;
-  if (nt * kRows >= p.N) return;
+  const int64_t kb = int64_t(blockIdx.x) * kPackBlocks + (threadIdx.x >> 6), nt = blockIdx.y + int64_t(blockIdx.z) * gridDim.y;
+  if (nt * kRows >= p.N || kb >= p.kblocks) return;
   uint8_t *block = p.packed + (nt * p.kblocks + kb) * p.bytes;
-  const int t = threadIdx.x, h = t >> 7, lane = (t >> 2) & 31, w = t & 3, r = lane >> 2, c = lane & 3;
-  const int64_t k0 = kb * kBlockK + 64 * h + 32 * (w >> 1) + 8 * c + 4 * (w & 1);
-  auto code = [&](int64_t n, int64_t k) -> uint32_t {
+  const int t = threadIdx.x & 63, h = t >> 5, lane = t & 31, r = lane >> 2, c = lane & 3;
+  // eight codes of output n from k (a multiple of 8): k + i at bits 4 i
+  auto codes8 = [&](int64_t n, int64_t k) -> uint32_t {
     if (n >= p.N || k >= p.K) return 0u;   // meets a scale or an x of zero
-    const uint32_t b = p.codes[n * p.codes_stride + (k >> 1)];
-    return (k & 1) ? b >> 4 : b & 15u;
+    const uint8_t *from = p.codes + n * p.codes_stride + (k >> 1);
+    if (k + 8 <= p.K && (reinterpret_cast<uintptr_t>(from) & 3) == 0) return *reinterpret_cast<const uint32_t *>(from);
+    uint32_t v = 0;
+    for (int i = 0; i < 4; ++i)
+      if (k + 2 * i < p.K) v |= uint32_t(from[i]) << (8 * i);
+    return v;
   };
-  uint32_t word = 0;
+  uint32_t word[4];
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    const int64_t n = nt * kRows + r + 8 * (s & 1), k = k0 + 2 * (s >> 1);
-    const uint32_t pair = code(n, k) | code(n, k + 1) << 16;
-    word |= s < 3 ? pair << (4 * s + 2) : (pair & 0x00030003u) << 14 | (pair >> 2 & 0x00030003u);
+  for (int u = 0; u < 2; ++u) {
+    const int64_t k = kb * kBlockK + 64 * h + 32 * u + 8 * c, n = nt * kRows + r;
+    const uint32_t row[2] = {codes8(n, k), codes8(n + 8, k)};
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      uint32_t out = 0;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const uint32_t two = row[s & 1] >> (16 * w + 8 * (s >> 1)), pair = (two & 15u) | (two & 0xF0u) << 12;
+        out |= s < 3 ? pair << (4 * s + 2) : (pair & 0x00030003u) << 14 | (pair >> 2 & 0x00030003u);
+      }
+      word[2 * u + w] = out;
+    }
   }
-  reinterpret_cast<uint32_t *>(block)[h * 128 + lane * 4 + w] = word;
+  reinterpret_cast<uint4 *>(block)[h * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
   if (t < p.gpb * kRows) {   // [output][group]
     const int64_t n = nt * kRows + t / p.gpb, g = (kb * kBlockK + int64_t(t % p.gpb) * (kBlockK / p.gpb)) / p.group;
     const bool in = n < p.N && g * p.group < p.K;
@@ -633,7 +647,8 @@ void w4_pack(const uint8_t *codes, int64_t codes_stride, const void *scales, int
   p.gpb = groups_per_block(group);
   p.bytes = block_bytes(group, zeros != nullptr);
   const int64_t tiles = (N + kRows - 1) / kRows, y = std::min<int64_t>(tiles, 32768);
-  w4_pack_kernel<<<dim3(unsigned(p.kblocks), unsigned(y), unsigned((tiles + y - 1) / y)), 256, 0, stream>>>(p);
+  const dim3 grid{unsigned((p.kblocks + kPackBlocks - 1) / kPackBlocks), unsigned(y), unsigned((tiles + y - 1) / y)};
+  w4_pack_kernel<<<grid, kPackBlocks * 64, 0, stream>>>(p);
   GCB_CUDA(cudaGetLastError());
   count_launch();
 }
