@@ -48,9 +48,10 @@ constexpr float kLazy = 8.f;
 // The workspace: a Cut for every block, then two parts for every block.  Part of a cut unit: [cols][dim] f32 sums, then m and l of
 // each column.
 struct Cut {
-  int64_t begin;         // the unit's first tile in the row of all tiles
-  int seq, unit, tiles;  // tiles 0: this border cuts nothing, or not as the first one
-  int per;
+  int seq, unit;
+  int first, count;      // blocks with a part of the unit; count 0: this border cuts nothing, or not as the first one
+  int place;             // of the first block's part: 1 if the unit begins inside its share, 0 with its share
+  int pad[3];
 };
 struct PagedAttParams {
   PagedCache c;
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
 
   const int64_t total = count_tiles<S::kTile>(p, units, pre), per = share_of(total, p.blocks, p.least);
   const int64_t begin = int64_t(blockIdx.x) * per, stop = min(total, begin + per);
-  Cut cut{0, 0, 0, 0, 0};
+  Cut cut{};
 
   if (begin < stop) {
     Place at = locate<S::kTile>(p, units, pre, begin, &found);
@@ -203,7 +204,14 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
     Cursor ahead = comp;   // of the tile whose page numbers are being fetched
     const int count = int(stop - begin);
     const int first_tile = comp.tile;
-    if (first_cut(blockIdx.x, per, begin - first_tile, begin - first_tile + comp.tiles)) cut = Cut{begin - first_tile, comp.seq, comp.unit, comp.tiles, int(per)};
+    const int64_t unit_begin = begin - first_tile;
+    if (first_cut(blockIdx.x, per, unit_begin, unit_begin + comp.tiles)) {   // the unit begins in the share of the block before
+      cut.seq = comp.seq;
+      cut.unit = comp.unit;
+      cut.first = int(blockIdx.x) - 1;
+      cut.count = int((unit_begin + comp.tiles - 1 - (begin - per)) / per) + 1;
+      cut.place = int(part_slot(cut.first, per, unit_begin) & 1);
+    }
 
     uint8_t *mine = smem + warp * kStages * S::kSlot;
     uint8_t *qring = smem + kWarps * kStages * S::kSlot;
@@ -605,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
 
 // Block (i - 1, y): the unit that border i cuts first; warp w of it column 4 y + w.  The lanes weigh 32 parts at a time by their
 // maxima, then add the parts up, four elements to a lane and eight parts under way.
-template <bool BF16, bool F8, int NT>
+template <bool BF16, bool F8, int NT, int HALVES>   // HALVES: of head_dim, 128 elements to the lanes at a time
 __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_constant__ PagedAttParams p) {
   constexpr int kCols = 8 * NT;
   const PagedCache &c = p.c;
@@ -613,21 +621,40 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
   pdl_wait();
   pdl_launch_dependents();
   const Cut cut = p.cuts[blockIdx.x + 1];
-  if (cut.tiles == 0) return;
+  const int count = cut.count;
+  if (count == 0) return;
   const int kv = cut.unit / p.sets, set = cut.unit - kv * p.sets;
   if (col >= min(kCols, p.group - set * kCols)) return;
-  const int b0 = int(cut.begin / cut.per), count = int((cut.begin + cut.tiles - 1) / cut.per) - b0 + 1;
   const int64_t floats = part_floats(kCols, dim);
-  // part i of the unit: the first block's second place if the unit begins there, every other block's first
-  const float *first = p.parts + part_slot(b0, cut.per, cut.begin) * floats, *rest = p.parts + 2 * int64_t(b0) * floats;
+  // part i of the unit: the first block's may lie in its second place, every other block's lies in its first
+  const float *rest = p.parts + 2 * int64_t(cut.first) * floats, *first = rest + cut.place * floats;
   auto part = [&](int i) { return i == 0 ? first : rest + 2 * int64_t(i) * floats; };
+  auto of_lane = [&](int i, int h) {   // this lane's four elements of part i
+    return i < count && h * 128 + lane * 4 < dim ? *reinterpret_cast<const float4 *>(part(i) + int64_t(col) * dim + h * 128 + lane * 4)
+                                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  // everything that a unit of up to eight parts needs is asked for at once
+  constexpr int kAhead = 8;
+  float4 ahead[kAhead][HALVES];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) ahead[i][h] = of_lane(i, h);
   float m = -INFINITY;
   for (int i = lane; i < count; i += 32) m = fmaxf(m, part(i)[int64_t(kCols) * dim + 2 * col]);
 #pragma unroll
   for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, i));
   const float ref = finite_ref(m);
   float l = 0.f;
-  float4 sum[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  float4 sum[HALVES];
+#pragma unroll
+  for (int h = 0; h < HALVES; ++h) sum[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](const float4 &v, float by, int h) {
+    sum[h].x = fmaf(v.x, by, sum[h].x);
+    sum[h].y = fmaf(v.y, by, sum[h].y);
+    sum[h].z = fmaf(v.z, by, sum[h].z);
+    sum[h].w = fmaf(v.w, by, sum[h].w);
+  };
   for (int i0 = 0; i0 < count; i0 += 32) {
     float w = 0.f;
     if (i0 + lane < count) {
@@ -636,19 +663,22 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
       l = fmaf(ml.y, w, l);
     }
     const int n = min(32, count - i0);
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-      const float by = __shfl_sync(0xFFFFFFFFu, w, i);
-      const float *from = part(i0 + i) + int64_t(col) * dim;
+    int i = 0;
+    if (i0 == 0) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (h * 128 + lane * 4 < dim) {
-          const float4 v = *reinterpret_cast<const float4 *>(from + h * 128 + lane * 4);
-          sum[h].x = fmaf(v.x, by, sum[h].x);
-          sum[h].y = fmaf(v.y, by, sum[h].y);
-          sum[h].z = fmaf(v.z, by, sum[h].z);
-          sum[h].w = fmaf(v.w, by, sum[h].w);
-        }
+      for (int a = 0; a < kAhead; ++a) {
+        const float by = __shfl_sync(0xFFFFFFFFu, w, a);
+        if (a < n)
+#pragma unroll
+          for (int h = 0; h < HALVES; ++h) add(ahead[a][h], by, h);
+      }
+      i = kAhead;
+    }
+#pragma unroll 8
+    for (; i < n; ++i) {
+      const float by = __shfl_sync(0xFFFFFFFFu, w, i);
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) add(of_lane(i0 + i, h), by, h);
     }
   }
 #pragma unroll
@@ -657,7 +687,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
   const int head = kv * p.group + set * kCols + col;
   uint16_t *out = p.out + cut.seq * p.o_seq + head * p.o_head;
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int h = 0; h < HALVES; ++h)
     if (h * 128 + lane * 4 < dim) {
       const float v[4] = {sum[h].x, sum[h].y, sum[h].z, sum[h].w};
 #pragma unroll
@@ -703,7 +733,7 @@ template <bool BF16, bool F8, int DP, int NT, bool FULL> void launch(PagedAttPar
   p.blocks = std::min(kMaxBlocks, dev.sm_count * r);
   p.least = 1;
   launch_dependent(kernel, dim3(unsigned(p.blocks)), S::kBytes, stream, p);
-  if (p.blocks > 1) launch_dependent(paged_join_kernel<BF16, F8, NT>, dim3(unsigned(p.blocks - 1), 2 * NT), 0, stream, p);
+  if (p.blocks > 1) launch_dependent(paged_join_kernel<BF16, F8, NT, (DP + 127) / 128>, dim3(unsigned(p.blocks - 1), 2 * NT), 0, stream, p);
 }
 
 template <bool BF16, bool F8> void launch(const PagedAttParams &p, int cols, DeviceState &dev, cudaStream_t stream) {
