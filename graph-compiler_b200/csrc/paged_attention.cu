@@ -633,13 +633,15 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
     return i < count && h * 128 + lane * 4 < dim ? *reinterpret_cast<const float4 *>(part(i) + int64_t(col) * dim + h * 128 + lane * 4)
                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
   };
-  // everything that a unit of up to eight parts needs is asked for at once
-  constexpr int kAhead = 8;
+  // everything that a unit of up to sixteen parts needs is asked for at once
+  constexpr int kAhead = 16;
   float4 ahead[kAhead][HALVES];
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i)
+  for (int i = 0; i < kAhead; ++i) {
+    if (i == kAhead / 2 && count <= kAhead / 2) break;
 #pragma unroll
     for (int h = 0; h < HALVES; ++h) ahead[i][h] = of_lane(i, h);
+  }
   float m = -INFINITY;
   for (int i = lane; i < count; i += 32) m = fmaxf(m, part(i)[int64_t(kCols) * dim + 2 * col]);
 #pragma unroll
@@ -667,6 +669,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
     if (i0 == 0) {
 #pragma unroll
       for (int a = 0; a < kAhead; ++a) {
+        if (a == kAhead / 2 && n <= kAhead / 2) break;
         const float by = __shfl_sync(0xFFFFFFFFu, w, a);
         if (a < n)
 #pragma unroll
