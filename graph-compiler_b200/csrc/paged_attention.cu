@@ -22,11 +22,12 @@
 //  * 8-bit caches become f16 in registers (exact).  Queries are scaled to f16 by a power of two per head.  (Queries as sums of e4m3
 //    numbers against the keys as they are, in e4m3 products, took 236 us where this takes 227.)
 //
-// Measured, 128-wide heads, eight query heads to a KV head unless said otherwise: 2 x 131071 tokens 174 us (6.2 TB/s; a copy reaches
-// 6.6), 64 x 512..4096 tokens with four heads to a KV head 103 (5.9), 16 x 2048 tokens of 32 heads of their own 90 (6.0), 128 x 1024..8192
-// tokens in 8 bits 205 (5.8, at the power cap: 620 instructions for 8 KB of cache against 340 in 16 bits).  Few tokens: 1 x 1031 takes
-// 11 us, most of it two launches on the host; 37 windows of up to 700 tokens 14 us, a chain of latencies (lengths, page numbers,
-// tokens, the warps' sums, the join).
+// Measured, 128-wide heads, eight query heads to a KV head unless said otherwise: 2 x 131071 tokens 168 us (6.4 TB/s; a copy reaches
+// 6.6), 64 x 512..4096 tokens with four heads to a KV head 101 (6.0), 16 x 2048 tokens of 32 heads of their own 87 (6.2), 128 x 1024..8192
+// tokens in 8 bits 195 (6.1, at the power cap: 620 instructions for 8 KB of cache against 340 in 16 bits); sixteen query heads to a
+// KV head, whose registers leave two blocks to an SM, 2 x 131071 214 (5.0).  Few tokens: 1 x 1031 takes 8.8 us, as much on the host (two
+// launches) as on the device; 37 windows of up to 700 tokens 12.4, a chain of latencies (lengths, page numbers, tokens, the warps'
+// sums, the join).
 #include "decode_ops.h"
 
 #include <algorithm>
@@ -634,6 +635,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
   };
   // everything that a unit of up to sixteen parts needs is asked for at once
+  // (one by one behind their weights, eight under way, the join of 17 parts took 2.3 us longer; eight asked for at once 1.2)
   constexpr int kAhead = 16;
   float4 ahead[kAhead][HALVES];
 #pragma unroll
