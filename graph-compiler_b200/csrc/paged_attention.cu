@@ -22,7 +22,7 @@
 //  * 8-bit caches become f16 in registers (exact).  Queries are scaled to f16 by a power of two per head.  (Queries as sums of e4m3
 //    numbers against the keys as they are, in e4m3 products, took 236 us where this takes 227.)
 //
-// Measured, 128-wide heads, eight query heads to a KV head unless said otherwise: 2 x 131071 tokens 168 us (6.4 TB/s; a copy reaches
+// Measured, 128-wide heads, eight query heads to a KV head unless said otherwise: 2 x 131071 tokens 166 us (6.4 TB/s; a copy reaches
 // 6.6), 64 x 512..4096 tokens with four heads to a KV head 101 (6.0), 16 x 2048 tokens of 32 heads of their own 87 (6.2), 128 x 1024..8192
 // tokens in 8 bits 195 (6.1, at the power cap: 620 instructions for 8 KB of cache against 340 in 16 bits); sixteen query heads to a
 // KV head, whose registers leave two blocks to an SM, 2 x 131071 214 (5.0).  Few tokens: 1 x 1031 takes 8.8 us, as much on the host (two
@@ -50,9 +50,10 @@ constexpr float kLazy = 8.f;
 // each column.
 struct Cut {
   int seq, unit;
-  int first, count;      // blocks with a part of the unit; count 0: this border cuts nothing, or not as the first one
+  int first, count;      // blocks with a part of the unit that the border before this block cuts; count 0: it cuts nothing
   int place;             // of the first block's part: 1 if the unit begins inside its share, 0 with its share
-  int pad[3];
+  int lead;              // the unit's first cut
+  int pad[2];
 };
 struct PagedAttParams {
   PagedCache c;
@@ -206,11 +207,12 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
     const int count = int(stop - begin);
     const int first_tile = comp.tile;
     const int64_t unit_begin = begin - first_tile;
-    if (first_cut(blockIdx.x, per, unit_begin, unit_begin + comp.tiles)) {   // the unit begins in the share of the block before
+    if (first_tile > 0) {
       cut.seq = comp.seq;
       cut.unit = comp.unit;
-      cut.first = int(blockIdx.x) - 1;
-      cut.count = int((unit_begin + comp.tiles - 1 - (begin - per)) / per) + 1;
+      cut.lead = first_cut(blockIdx.x, per, unit_begin, unit_begin + comp.tiles);
+      cut.first = int(unit_begin / per);
+      cut.count = int((unit_begin + comp.tiles - 1) / per) - cut.first + 1;
       cut.place = int(part_slot(cut.first, per, unit_begin) & 1);
     }
 
@@ -612,31 +614,36 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
   }
 }
 
-// Block (i - 1, y): the unit that border i cuts first; warp w of it column 4 y + w.  The lanes weigh 32 parts at a time by their
-// maxima, then add the parts up, four elements to a lane and eight parts under way.
+// Block (i - 1, y): the unit that border i cuts.  Up to sixteen parts: the blocks of its first cut join them, a warp to a column.  More:
+// the blocks of all its cuts take a column each, the four warps every fourth part (156 parts behind one warp took 15 us).  The lanes
+// weigh 32 parts at a time by their maxima, then add the parts up, four elements to a lane.
 template <bool BF16, bool F8, int NT, int HALVES>   // HALVES: of head_dim, 128 elements to the lanes at a time
 __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_constant__ PagedAttParams p) {
   constexpr int kCols = 8 * NT;
   const PagedCache &c = p.c;
-  const int lane = threadIdx.x & 31, col = int(blockIdx.y) * kWarps + int(threadIdx.x >> 5), dim = c.dim;
+  __shared__ __align__(16) float warp_m[kWarps], warp_l[kWarps], warp_sum[kWarps][HALVES * 128];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = c.dim;
   pdl_wait();
   pdl_launch_dependents();
   const Cut cut = p.cuts[blockIdx.x + 1];
-  const int count = cut.count;
-  if (count == 0) return;
+  constexpr int kAhead = 16;   // parts asked for at once (one by one behind their weights, eight under way, 17 parts took 2.3 us longer)
+  const bool together = cut.count > kAhead;
+  if (cut.count == 0 || (!together && !cut.lead)) return;
   const int kv = cut.unit / p.sets, set = cut.unit - kv * p.sets;
+  const int col = together ? (int(blockIdx.x) - cut.first) * int(gridDim.y) + int(blockIdx.y) : int(blockIdx.y) * kWarps + warp;
   if (col >= min(kCols, p.group - set * kCols)) return;
+  const int step = together ? kWarps : 1, start = together ? warp : 0, count = (cut.count - start + step - 1) / step;   // this warp's parts
   const int64_t floats = part_floats(kCols, dim);
   // part i of the unit: the first block's may lie in its second place, every other block's lies in its first
   const float *rest = p.parts + 2 * int64_t(cut.first) * floats, *first = rest + cut.place * floats;
-  auto part = [&](int i) { return i == 0 ? first : rest + 2 * int64_t(i) * floats; };
+  auto part = [&](int i) {
+    const int at = start + i * step;
+    return at == 0 ? first : rest + 2 * int64_t(at) * floats;
+  };
   auto of_lane = [&](int i, int h) {   // this lane's four elements of part i
     return i < count && h * 128 + lane * 4 < dim ? *reinterpret_cast<const float4 *>(part(i) + int64_t(col) * dim + h * 128 + lane * 4)
                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
   };
-  // everything that a unit of up to sixteen parts needs is asked for at once
-  // (one by one behind their weights, eight under way, the join of 17 parts took 2.3 us longer; eight asked for at once 1.2)
-  constexpr int kAhead = 16;
   float4 ahead[kAhead][HALVES];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
@@ -688,6 +695,28 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
   }
 #pragma unroll
   for (int i = 16; i > 0; i >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, i);
+  if (together) {
+    if (lane == 0) {
+      warp_m[warp] = m;
+      warp_l[warp] = l;
+    }
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) *reinterpret_cast<float4 *>(&warp_sum[warp][h * 128 + lane * 4]) = sum[h];
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) m = fmaxf(m, warp_m[w]);
+    l = 0.f;
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) sum[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float by = ex2(warp_m[w] - finite_ref(m));
+      l = fmaf(warp_l[w], by, l);
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) add(*reinterpret_cast<const float4 *>(&warp_sum[w][h * 128 + lane * 4]), by, h);
+    }
+  }
   const float scale = (F8 && c.value_scale ? c.value_scale[kv] : 1.f) / l;
   const int head = kv * p.group + set * kCols + col;
   uint16_t *out = p.out + cut.seq * p.o_seq + head * p.o_head;
@@ -698,7 +727,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
 #pragma unroll
       for (int e = 0; e < 4; ++e) out[h * 128 + lane * 4 + e] = f32_to_half<BF16>(v[e] * scale);
     }
-  if (lane == 0 && p.lse) p.lse[int64_t(cut.seq) * p.heads + head] = (ref + log2f(l)) * 0.6931471805599453f;
+  if (lane == 0 && p.lse) p.lse[int64_t(cut.seq) * p.heads + head] = (finite_ref(m) + log2f(l)) * 0.6931471805599453f;
 }
 
 void require(bool ok, const char *what) {

@@ -162,6 +162,13 @@ def test_attention_many_sequences():
     _attend_check("f16", "e4m3", [int(x) for x in r.randint(0, 20, 700)], 2, 1, 64, 16)
 
 
+@pytest.mark.parametrize("dim,heads", [(256, 3), (176, 9), (128, 12), (64, 1)])
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_attention_many_parts_to_a_unit(dim, heads, kind):
+    """One KV head, a long sequence beside short ones: its softmax is cut by dozens of borders."""
+    _attend_check("bf16", kind, [2500, 3, 0, 1400, 64], heads, 1, dim, 16, seed=dim)
+
+
 def test_attention_more_sequences_than_a_grid_has_rows():
     """Seventy thousand sequences of one token, every seventh empty: each gives its own value row, bit for bit."""
     S, D = 70000, 16
