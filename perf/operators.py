@@ -24,17 +24,13 @@ DEV = "cuda"
 DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "e4m3": torch.float8_e4m3fn}
 
 
-_module = None
-
-
 def _lib():
-    global _module
-    if _module is None:   # a program imports the library once
-        sys.path.insert(0, os.path.abspath("graph-compiler_b200"))
-        from gc_b200 import lib
+    path = os.path.abspath("graph-compiler_b200")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from gc_b200 import lib
 
-        _module = lib
-    return _module
+    return lib
 
 
 # ----------------------------------------------------------------------------- cases
