@@ -72,7 +72,14 @@ GCB_EXPORT const char *gcb200_last_error(void) { return g_last_error.c_str(); }
 GCB_EXPORT int gcb200_device_error(void *stream, int *code) {
   return guarded([&] {
     require(code != nullptr, "code is null");
-    *code = read_device_error(static_cast<cudaStream_t>(stream));
+    *code = read_device_error(static_cast<cudaStream_t>(stream), false);
+  });
+}
+
+GCB_EXPORT int gcb200_wait_error(void *stream, int *code) {
+  return guarded([&] {
+    require(code != nullptr, "code is null");
+    *code = read_device_error(static_cast<cudaStream_t>(stream), true);
   });
 }
 

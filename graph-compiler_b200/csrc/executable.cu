@@ -766,8 +766,7 @@ struct dnnl_graph_compiler_executable {
       if (piped_out >= 0) GCB_CUDA(cudaStreamSynchronize(copy_out));
       if (const int code = device_state().take_error()) {
         gcLogE("device error word = ", code, " after execute");
-        throw std::runtime_error(code == ERR_BAD_PAGE ? std::string("a call on a paged cache met a page number or a length outside the cache (code 9)")
-                                                      : "a kernel gave up a bounded wait (code " + std::to_string(code) + ")");
+        throw std::runtime_error("a kernel gave up a bounded wait (code " + std::to_string(code) + ")");
       }
       for (size_t i = 0; i < no; ++i)
         if (out_user[i]) std::memcpy(out_user[i], out_ptr[i], size_t(p.tensors.at(p.output_ids[i]).numel()) * dtype_bytes(p.tensors.at(p.output_ids[i]).dtype));

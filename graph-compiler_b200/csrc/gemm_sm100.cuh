@@ -18,7 +18,7 @@ enum ErrCode : int {
   ERR_WAIT_PEER = 6,       // a cross-GPU counter (rows landed / partial sums landed) never reached its target
   ERR_WAIT_PARTS = 8,      // few-rows form: a CTA of the cluster never handed over its partial sums
   ERR_SELFTEST = 7,        // the wait self-test: a wait nobody satisfies ran out, as intended
-  ERR_BAD_PAGE = 9,        // paged cache: a page number or a length outside the cache
+  ERR_BAD_PAGE = 9,        // paged cache: a page number or a length outside the cache (in a word of its own)
 };
 
 // Geometry of one operand's pipeline stage in shared memory and of the

@@ -283,7 +283,7 @@ void paged_kv_append(const gcb200_paged_cache &cache, const AppendArgs &a, cudaS
           "paged append: rotary_dim must be even and at most head_dim (0 without inv_freq)");
   if (a.tokens == 0) return;
   DeviceState &dev = device_state();
-  p.c.error = dev.d_error;
+  p.c.error = dev.d_page_error;
   p.q = static_cast<const uint16_t *>(a.q);
   p.k = static_cast<const uint16_t *>(a.k);
   p.v = static_cast<const uint16_t *>(a.v);

@@ -797,7 +797,7 @@ void paged_attention(const gcb200_paged_cache &cache, const PagedAttentionArgs &
   require(a.window >= 0, "paged attention: negative window");
   if (cache.sequences == 0) return;
   DeviceState &dev = device_state();
-  p.c.error = dev.d_error;
+  p.c.error = dev.d_page_error;
   p.q = static_cast<const uint16_t *>(a.q);
   p.out = static_cast<uint16_t *>(a.out);
   p.q_seq = cache.sequences > 1 ? a.q_stride[0] : 0;

@@ -39,6 +39,7 @@ DeviceState &device_state() {
     d.sm_count = prop.multiProcessorCount;
     GCB_CUDA(cudaHostAlloc(reinterpret_cast<void **>(&d.d_error), 64, cudaHostAllocMapped | cudaHostAllocPortable));
     std::memset(d.d_error, 0, 64);
+    d.d_page_error = d.d_error + 8;
     GCB_CUDA(cudaMalloc(&d.d_zero, 64));
     GCB_CUDA(cudaMemset(d.d_zero, 0, 64));
     d.device = dev;
@@ -62,10 +63,11 @@ void *DeviceState::ensure_workspace(size_t bytes) {
   return workspace;
 }
 
-int read_device_error(cudaStream_t stream) {
+int read_device_error(cudaStream_t stream, bool waits_only) {
   DeviceState &d = device_state();
   GCB_CUDA(cudaStreamSynchronize(stream));
-  return d.take_error();
+  const int code = d.take_error();
+  return code || waits_only ? code : d.take_page_error();
 }
 
 // ----------------------------------------------------------------------------- tensor maps

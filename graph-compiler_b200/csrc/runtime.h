@@ -33,8 +33,13 @@ struct DeviceState {
   // touch it only when they give up, and after a stream synchronisation the host reads it without a copy (a copy behind
   // every synchronous call cost 4 us).
   int *d_error = nullptr;
-  int take_error() {               // reads and clears; the kernels in question must have completed
-    volatile int *w = d_error;
+  // The same for a caller's data: a page number or a length outside a paged cache, met by a call that has long returned.  A word of
+  // its own, so that no other call takes it for a failure of its own and no code of a wait is lost under it.
+  int *d_page_error = nullptr;
+  // These read and clear; the kernels in question must have completed.
+  int take_error() { return take(d_error); }
+  int take_page_error() { return take(d_page_error); }
+  static int take(volatile int *w) {
     const int code = *w;
     if (code) *w = 0;
     return code;
@@ -169,7 +174,8 @@ void matmul_bf16_packed(const MatmulArgs &a, void *pack, cudaStream_t stream);
 // The same with the copies in stream-ordered memory of this library's own pool (direct launchers: any stream, any thread).
 void matmul_bf16_any_layout(const MatmulArgs &a, cudaStream_t stream);
 
-int read_device_error(cudaStream_t stream); // synchronises the stream; returns and clears the error word
+// Synchronises the stream; returns and clears the code of a wait that gave up, or, behind that one, of a paged cache.
+int read_device_error(cudaStream_t stream, bool waits_only);
 
 // Kernel launches issued by this library since load (every launcher counts its own).
 // Sum `nparts` f32 planes of a [rows, N] slice in plane order, bias + ReLU + cast, and store the bf16 slice

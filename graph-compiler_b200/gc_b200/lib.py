@@ -65,6 +65,7 @@ def load() -> C.CDLL:
     lib.gcb200_last_error.restype = C.c_char_p
     sig = {
         "gcb200_device_error": [_vp, C.POINTER(_int)],
+        "gcb200_wait_error": [_vp, C.POINTER(_int)],
         "gcb200_sm_count": [C.POINTER(_int)],
         "gcb200_launch_count": [C.POINTER(_u64)],
         "gcb200_matmul_bf16_splitk_static": [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp],
@@ -190,6 +191,13 @@ def launch_count() -> int:
 def device_error() -> int:
     code = _int(0)
     check(load().gcb200_device_error(_stream(), C.byref(code)))
+    return code.value
+
+
+def wait_error() -> int:
+    """Like :func:`device_error`, but only of bounded waits: what a call on a paged cache has recorded (9) stays."""
+    code = _int(0)
+    check(load().gcb200_wait_error(_stream(), C.byref(code)))
     return code.value
 
 

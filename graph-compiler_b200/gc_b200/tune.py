@@ -123,7 +123,7 @@ def tune_matmul(M: int, N: int, K: int, int8: bool = False, iters: int = 10, rec
             results.append((repr(c), us))
             if us == us and us < best_us:
                 best, best_us = c, us
-        if lib.device_error() != 0:
+        if lib.wait_error() != 0:
             raise RuntimeError("a kernel reported a wait time-out while tuning")
     finally:
         if saved is not None:                              # leave the cache as it was unless a winner is recorded below

@@ -39,8 +39,12 @@ typedef enum {
 const char *gcb200_last_error(void);
 
 /* Reads and clears the device-side error word (0 = none; otherwise the code of
- * the bounded wait that gave up).  Synchronises `stream`. */
+ * the bounded wait that gave up).  Synchronises `stream`.  Where no wait gave up it
+ * reads and clears what calls on a paged cache have recorded (code 9, a page number
+ * or a length outside the cache); that is kept apart, and no other call fails for it. */
 int gcb200_device_error(void *stream, int *code);
+/* The same for bounded waits alone: a recorded code 9 stays. */
+int gcb200_wait_error(void *stream, int *code);
 
 /* Kernel launches this library has issued since it was loaded (all launchers,
  * all threads).  Benchmarks difference it around a timed region. */
@@ -205,7 +209,7 @@ int gcb200_attention_bf16(const void *Q, const void *K, const void *V, void *O, 
  * entries behind its last token are not read.  head_dim is a multiple of 8 (of 16 for 8-bit caches), at most 256; the
  * caches' base addresses and strides are multiples of 16 bytes.  cache_dtype is dtype, or GCB200_F8_E4M3: a cached number is
  * then code * scale of its KV head.  A page number outside [0, pages) that a call meets is never followed: the call records
- * code 9 in the device error word (gcb200_device_error), and those tokens count as zeros (attention) or are not written
+ * code 9, which gcb200_device_error returns, and those tokens count as zeros (attention) or are not written
  * (append).  Calls may be captured into a graph, once any call of this library has run on the device; a replay follows the page
  * table, positions and lengths that device memory holds then. */
 typedef enum { GCB200_F16 = 1, GCB200_BF16 = 2, GCB200_F8_E4M3 = 10 } gcb200_dtype; /* dnnl_data_type_t's codes where it has one */
@@ -239,7 +243,7 @@ int gcb200_paged_kv_append(const gcb200_paged_cache *cache, const void *q, const
  * lengths (device) count the tokens in the cache, the new one among them.  A sequence of length 0 (or less) gives zeros, and
  * minus infinity in lse.  lse [sequences][heads] f32 (may be NULL) receives log sum_t exp(scale * q . k_t).  Scores, maxima, sums
  * and results are held in f32; exp() of the scores is rounded to 16 bits (like the values it multiplies) and the result once.
- * A length beyond max_pages * page_size is cut to that and recorded as code 9 in the device error word.
+ * A length beyond max_pages * page_size is cut to that and recorded as code 9.
  * workspace: device memory, gcb200_paged_attention_workspace() bytes, 16-byte aligned, that no other call in flight uses; nothing
  * in it needs clearing or is kept from one call to the next. */
 int gcb200_paged_attention_workspace(int64_t heads, int64_t kv_heads, int64_t head_dim, size_t *bytes);
