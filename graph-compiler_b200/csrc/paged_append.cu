@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kAppendThreads<VEC>) append_kernel(const __gri
     turn[i] = make_float2(co, s);
   }
   const int slot = pos % c.table.page_size, page = page_of(c.table, seq, pos);
-  if (page < 0 && threadIdx.x == 0) atomicExch(c.error, int(ERR_BAD_PAGE));
+  if (page < 0 && threadIdx.x == 0) report_bad_page(c.error);
   __syncthreads();
   // this piece's pairs: element i of one chunk and of the other, or neighbours within a chunk
   float cs[VEC], sn[VEC];

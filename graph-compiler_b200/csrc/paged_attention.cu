@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
       next_page = -1;
       if (lane < S::kTokens && pos < ahead.end) {
         next_page = page_at(c.table, ahead.seq, entry);
-        if (next_page < 0) atomicExch(c.error, int(ERR_BAD_PAGE));
+        if (next_page < 0) report_bad_page(c.error);
       }
       entry += step_entry;
       slot += step_slot;
@@ -603,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
   // ---- sequences of which nothing is seen
   for (int s = blockIdx.x; s < c.table.sequences; s += gridDim.x) {
     const Seen see = seen_of(c.table, p.lengths[s], p.window);
-    if (see.cut && threadIdx.x == 0) atomicExch(c.error, int(ERR_BAD_PAGE));
+    if (see.cut && threadIdx.x == 0) report_bad_page(c.error);
     if (see.end > see.first) continue;
     for (int i = threadIdx.x; i < p.heads * dim; i += kThreads) {
       const int h = i / dim;

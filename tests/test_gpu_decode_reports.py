@@ -76,3 +76,39 @@ def test_a_long_row_of_bad_pages():
     out = lib.paged_attention(q, keys, keys, table, lens, 1.0, lse=lse)
     assert lib.device_error() == 9 and lib.device_error() == 0
     assert not out.any() and np.allclose(lse.cpu().numpy(), np.log(n), rtol=0, atol=2.0 ** -19)
+
+
+def _us(call, n=5):
+    call()
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    for _ in range(n):
+        call()
+    b.record()
+    torch.cuda.synchronize()
+    return a.elapsed_time(b) / n * 1e3
+
+
+def test_bad_pages_and_lengths_cost_no_more_than_good_ones():
+    """The code is recorded in host memory; a wait for the host at every token, sequence or thread would take 5000 times as long.  The
+    bound leaves room for a loaded host: the good calls take 20 to 100 us."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    H, D, page, n = 8, 128, 16, 16384
+    keys = torch.randn(2 * n // page, H, page, D, device="cuda", generator=g).bfloat16()
+    q, lens = torch.randn(2, H, D, device="cuda", generator=g).bfloat16(), torch.full((2,), n, dtype=torch.int32, device="cuda")
+    good = torch.arange(2 * n // page, dtype=torch.int32, device="cuda").view(2, -1)
+    bad = torch.full_like(good, -1)
+    attend = [_us(lambda: lib.paged_attention(q, keys, keys, t, lens, 1.0)) for t in (good, bad)]
+
+    x, other = torch.randn(n, H, D, device="cuda", generator=g).bfloat16(), torch.empty_like(keys)
+    seq, pos = torch.zeros(n, dtype=torch.int32, device="cuda"), torch.arange(n, dtype=torch.int32, device="cuda")
+    append = [_us(lambda: lib.paged_kv_append(None, x, x, keys, other, t, pos, sequences=seq)) for t in (good, bad)]
+
+    S = 70000
+    many, short, ones = torch.randn(S, 1, 16, device="cuda", generator=g).bfloat16(), torch.zeros(S, 1, dtype=torch.int32, device="cuda"), torch.ones(S, dtype=torch.int32, device="cuda")
+    small = torch.randn(1, 1, 1, 16, device="cuda", generator=g).bfloat16()
+    lengths = [_us(lambda: lib.paged_attention(many, small, small, short, lens, 1.0)) for lens in (ones, ones + 1)]
+    assert lib.device_error() == 9
+    for name, (right, wrong) in (("attention", attend), ("append", append), ("lengths", lengths)):
+        assert wrong < 50 * max(right, 20.0), (name, right, wrong)
