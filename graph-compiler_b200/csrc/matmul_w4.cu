@@ -599,7 +599,7 @@ void matmul_w4(int dtype, const void *X, int64_t ldx, const void *packed, const 
                int64_t N, int64_t K, int64_t group, int has_zeros, int relu, cudaStream_t stream) {
   checked_w4(N, K, group);
   require(dtype == GCB200_BF16 || dtype == GCB200_F16, "4-bit weights: x must be bf16 or f16");
-  require(M >= 0 && M <= 8 * 65535, "4-bit weights: number of rows out of range");
+  require(M >= 0 && M < (int64_t(1) << 31), "4-bit weights: number of rows out of range");
   if (M == 0) return;
   require(X && packed && Y, "4-bit weights: null pointer");
   require((reinterpret_cast<uintptr_t>(packed) & 15) == 0, "4-bit weights: the packed buffer must be 16-byte aligned");
@@ -610,15 +610,12 @@ void matmul_w4(int dtype, const void *X, int64_t ldx, const void *packed, const 
   W4Plan plan{};
   if (!plan_w4(int(M), tiles, kblocks, gpb, bytes, clusters_at_once(dev), &plan)) throw std::logic_error("4-bit weights: a row of x does not fit into the shared memory of a cluster");
   W4Params p{};
-  p.x = static_cast<const uint16_t *>(X);
   p.bias = static_cast<const uint16_t *>(bias);
   p.packed = static_cast<const uint8_t *>(packed);
-  p.y = static_cast<uint16_t *>(Y);
   p.ldx = M > 1 ? ldx : 0;
   p.ldy = M > 1 ? ldy : 0;
   p.N = N;
   p.K = K;
-  p.M = int(M);
   p.pass = plan.pass;
   p.relu = relu;
   p.kblocks = kblocks;
@@ -632,14 +629,19 @@ void matmul_w4(int dtype, const void *X, int64_t ldx, const void *packed, const 
   p.meet_at = plan.meet_at;
   p.part_at = plan.part_at;
   p.error = dev.d_error;
-  const int grid_y = int((M + plan.pass - 1) / plan.pass);
-  require(grid_y <= 65535, "4-bit weights: number of rows out of range");
-  auto go = [&](auto bf16) {
-    constexpr bool B = decltype(bf16)::value;
-    if (plan.nt == 1) plan.rt == 2 ? launch<B, 1, 2>(p, plan, gpb, has_zeros != 0, grid_y, dev.device, stream) : launch<B, 1, 1>(p, plan, gpb, has_zeros != 0, grid_y, dev.device, stream);
-    else plan.rt == 2 ? launch<B, 2, 2>(p, plan, gpb, has_zeros != 0, grid_y, dev.device, stream) : launch<B, 2, 1>(p, plan, gpb, has_zeros != 0, grid_y, dev.device, stream);
-  };
-  dtype == GCB200_BF16 ? go(std::true_type{}) : go(std::false_type{});
+  const int64_t most = int64_t(65535) * plan.pass;   // rows of a launch: a grid has that many passes
+  for (int64_t m = 0; m < M; m += most) {
+    p.x = static_cast<const uint16_t *>(X) + m * p.ldx;
+    p.y = static_cast<uint16_t *>(Y) + m * p.ldy;
+    p.M = int(std::min(most, M - m));
+    const int grid_y = (p.M + plan.pass - 1) / plan.pass;
+    auto go = [&](auto bf16) {
+      constexpr bool B = decltype(bf16)::value;
+      if (plan.nt == 1) plan.rt == 2 ? launch<B, 1, 2>(p, plan, gpb, has_zeros != 0, grid_y, dev.device, stream) : launch<B, 1, 1>(p, plan, gpb, has_zeros != 0, grid_y, dev.device, stream);
+      else plan.rt == 2 ? launch<B, 2, 2>(p, plan, gpb, has_zeros != 0, grid_y, dev.device, stream) : launch<B, 2, 1>(p, plan, gpb, has_zeros != 0, grid_y, dev.device, stream);
+    };
+    dtype == GCB200_BF16 ? go(std::true_type{}) : go(std::false_type{});
+  }
 }
 
 } // namespace gcb

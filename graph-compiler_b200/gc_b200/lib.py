@@ -508,7 +508,9 @@ def pack_w4(codes, scales, K: int, group: int, zeros=None) -> W4Weights:
 
 
 def matmul_w4(x, weights: W4Weights, bias=None, relu: bool = False, out=None):
-    """act(x . W^T + bias) for a few rows: x ``[M, K]`` of the scales' type, f32 products and sums, rounded once."""
+    """act(x . W^T + bias) for a few rows: x ``[M, K]`` of the scales' type, f32 products and sums, rounded once.
+
+    K is at most 195584.  More rows than 16 (fewer for K > 22528) read the weights again."""
     w = weights
     if out is None:
         import torch

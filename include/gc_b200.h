@@ -259,8 +259,9 @@ int gcb200_paged_attention(const gcb200_paged_cache *cache, const void *q, const
  * group is 32, 64 or a multiple of 128.  gcb200_w4_pack lays the weights out once, in the order in which the kernel reads them:
  * codes [N] rows of (K + 1) / 2 bytes (even k in the low half of a byte), scales and zeros [N][ceil(K / group)] (zeros NULL: 8);
  * row strides are in elements.  packed: gcb200_w4_packed_bytes() bytes, 16-byte aligned.  The scales' type is that of the X the
- * weights will meet.  Y may not overlap X.  Any M; more than 16 rows read the weights once for every 16.  NaN or an infinity in a row of X makes that
- * row's results NaN, and no other's. */
+ * weights will meet.  Y may not overlap X.  Any M below 2^31: the weights are read once for every 16 rows up to K = 22528, every 8 up
+ * to 43008, every 4 up to 77824, every 2 up to 130048, and for every row up to 195584, the longest K (GCB200_UNIMPLEMENTED beyond,
+ * from the product, not from the packing).  NaN or an infinity in a row of X makes that row's results NaN, and no other's. */
 int gcb200_w4_packed_bytes(int64_t N, int64_t K, int64_t group, int has_zeros, size_t *bytes);
 int gcb200_w4_pack(const uint8_t *codes, int64_t codes_stride, const void *scales, int64_t scales_stride, const uint8_t *zeros,
                    int64_t zeros_stride, int64_t N, int64_t K, int64_t group, void *packed, void *stream);
