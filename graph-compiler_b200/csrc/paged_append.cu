@@ -278,6 +278,7 @@ void paged_kv_append(const gcb200_paged_cache &cache, const AppendArgs &a, cudaS
   require(!a.q || a.q_out, "paged append: queries without a place to go");
   require(a.tokens >= 0 && a.tokens < (int64_t(1) << 31), "paged append: number of tokens out of range");
   require(!a.q || (a.heads > 0 && a.heads < 65536), "paged append: number of heads out of range");
+  require(!a.q || !rows_overlap(a.tokens, a.q_out_stride[0], a.heads, a.q_out_stride[1], cache.head_dim), "paged append: rows of the rotated queries overlap");
   require(a.sequences || a.tokens <= cache.sequences, "paged append: more tokens than sequences, and no sequence numbers");
   require(a.inv_freq ? a.rotary_dim >= 2 && a.rotary_dim % 2 == 0 && a.rotary_dim <= cache.head_dim : a.rotary_dim == 0,
           "paged append: rotary_dim must be even and at most head_dim (0 without inv_freq)");

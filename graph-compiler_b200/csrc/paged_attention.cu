@@ -795,6 +795,7 @@ void paged_attention(const gcb200_paged_cache &cache, const PagedAttentionArgs &
   require((reinterpret_cast<uintptr_t>(a.workspace) & 15) == 0, "paged attention: the workspace must be 16-byte aligned");
   require(a.workspace_bytes >= paged_attention_workspace(a.heads, cache.kv_heads, cache.head_dim), "paged attention: the workspace is too small");
   require(a.window >= 0, "paged attention: negative window");
+  require(!rows_overlap(cache.sequences, a.out_stride[0], a.heads, a.out_stride[1], cache.head_dim), "paged attention: rows of the result overlap");
   if (cache.sequences == 0) return;
   DeviceState &dev = device_state();
   p.c.error = dev.d_page_error;

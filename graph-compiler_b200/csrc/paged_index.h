@@ -26,6 +26,27 @@ GCB_HD int page_at(const PageTable &t, int seq, int entry) {
 // Page that holds position `pos`.
 GCB_HD int page_of(const PageTable &t, int seq, int pos) { return pos < 0 ? -1 : page_at(t, seq, pos / t.page_size); }
 
+// Whether two of the rows of `dim` elements at i a + j b overlap (0 <= i < na, 0 <= j < nb).
+inline bool rows_overlap(int64_t na, int64_t a, int64_t nb, int64_t b, int64_t dim) {
+  if (na < 1 || nb < 1) return false;
+  if (na == 1) na = nb, a = b, nb = 1;
+  if (na == 1) return false;
+  a = a < 0 ? -a : a;   // the same rows, counted from the other end
+  b = b < 0 ? -b : b;
+  if (nb > 1 && a > b) {
+    int64_t t = a; a = b; b = t;
+    t = na; na = nb; nb = t;
+  }
+  if (a < dim) return true;
+  // rows i and j steps away: the nearest ones before and behind every j b
+  for (int64_t j = 1; j < nb; ++j) {
+    const int64_t i = j * b / a, rest = j * b - i * a;
+    if (i >= na) return false;
+    if (rest < dim || (i + 1 < na && a - rest < dim)) return true;
+  }
+  return false;
+}
+
 // Positions [first, end) that a query sees in a sequence said to hold `length` tokens; window 0: all.  `cut`: length was more than
 // the table has room for.
 struct Seen {
