@@ -11,6 +11,9 @@
 
 namespace gcb {
 
+// Whether an address (or none) is a multiple of `bytes`: the kernels would stop at any other with a fault.
+inline bool aligned(const void *p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
 // What the kernels of the cache see.  Strides in bytes.
 struct PagedCache {
   uint8_t *keys, *values;

@@ -603,6 +603,7 @@ void matmul_w4(int dtype, const void *X, int64_t ldx, const void *packed, const 
   if (M == 0) return;
   require(X && packed && Y, "4-bit weights: null pointer");
   require((reinterpret_cast<uintptr_t>(packed) & 15) == 0, "4-bit weights: the packed buffer must be 16-byte aligned");
+  require(aligned(X, 2) && aligned(bias, 2) && aligned(Y, 2), "4-bit weights: misaligned pointer");
   require(M == 1 || (ldx >= K && ldy >= N), "4-bit weights: rows overlap");
   DeviceState &dev = device_state();
   const int kblocks = int((K + kBlockK - 1) / kBlockK), tiles = int((N + kRows - 1) / kRows);

@@ -258,6 +258,7 @@ PagedCache checked_cache(const gcb200_paged_cache &c, bool writes) {
     if (writes && extent[i] > 1) require(ks[i] >= c.head_dim * size && vs[i] >= c.head_dim * size, "paged cache: rows of the cache overlap");
   }
   require(((reinterpret_cast<uintptr_t>(c.keys) | reinterpret_cast<uintptr_t>(c.values)) & 15) == 0, "paged cache: keys and values must be 16-byte aligned");
+  require(aligned(c.page_table, 4) && aligned(c.key_scale, 4) && aligned(c.value_scale, 4), "paged cache: misaligned page table or scales");
   PagedCache d{};
   d.keys = static_cast<uint8_t *>(c.keys);
   d.values = static_cast<uint8_t *>(c.values);
@@ -282,6 +283,8 @@ void paged_kv_append(const gcb200_paged_cache &cache, const AppendArgs &a, cudaS
   require(a.sequences || a.tokens <= cache.sequences, "paged append: more tokens than sequences, and no sequence numbers");
   require(a.inv_freq ? a.rotary_dim >= 2 && a.rotary_dim % 2 == 0 && a.rotary_dim <= cache.head_dim : a.rotary_dim == 0,
           "paged append: rotary_dim must be even and at most head_dim (0 without inv_freq)");
+  require(aligned(a.q, 2) && aligned(a.k, 2) && aligned(a.v, 2) && aligned(a.q_out, 2) && aligned(a.sequences, 4) && aligned(a.positions, 4) && aligned(a.inv_freq, 8),
+          "paged append: misaligned pointer");
   if (a.tokens == 0) return;
   DeviceState &dev = device_state();
   p.c.error = dev.d_page_error;

@@ -796,6 +796,7 @@ void paged_attention(const gcb200_paged_cache &cache, const PagedAttentionArgs &
   require(a.workspace_bytes >= paged_attention_workspace(a.heads, cache.kv_heads, cache.head_dim), "paged attention: the workspace is too small");
   require(a.window >= 0, "paged attention: negative window");
   require(!rows_overlap(cache.sequences, a.out_stride[0], a.heads, a.out_stride[1], cache.head_dim), "paged attention: rows of the result overlap");
+  require(aligned(a.q, 2) && aligned(a.out, 2) && aligned(a.lengths, 4) && aligned(a.lse, 4), "paged attention: misaligned pointer");
   if (cache.sequences == 0) return;
   DeviceState &dev = device_state();
   p.c.error = dev.d_page_error;

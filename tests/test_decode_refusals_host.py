@@ -1,4 +1,5 @@
-"""Refusals of the decode operators without a device: results whose rows overlap, on which several thread blocks would write at once."""
+"""Refusals of the decode operators without a device: results whose rows overlap, on which several thread blocks would write at once, and addresses at which
+a kernel would stop with a fault."""
 import ctypes as C
 import os
 import subprocess
@@ -46,3 +47,22 @@ def test_results_whose_rows_overlap_are_refused(stride):
     assert b"overlap" in l.gcb200_last_error()
     assert l.gcb200_paged_kv_append(C.byref(d), P, s, 4, P, s, P, s, P, o, None, P, 3, None, 0, 0, None) == INVALID
     assert b"overlap" in l.gcb200_last_error()
+
+
+def test_misaligned_addresses_are_refused():
+    l, s, n = lib.load(), _i64s(256, 64), 0
+    attend = [P, s, 4, P, 1.0, 0, P, s, P, P, 1 << 30, None]
+    append = [P, s, 4, P, s, P, s, P, s, P, P, 3, P, 64, 0, None]
+    matmul = [2, P, 128, P, P, P, 16, 2, 16, 128, 128, 0, 0, None]
+    descs = [_desc(page_table=P + 2), _desc(cache_dtype=10, key_scale=P + 1), _desc(cache_dtype=10, value_scale=P + 2)]
+    for d in descs:
+        assert l.gcb200_paged_attention(C.byref(d), *attend) == INVALID and l.gcb200_paged_kv_append(C.byref(d), *append) == INVALID
+    for call, good, at in ((l.gcb200_paged_attention, [C.byref(_desc())] + attend, {1: 1, 4: 2, 7: 1, 9: 2}),
+                           (l.gcb200_paged_kv_append, [C.byref(_desc())] + append, {1: 1, 4: 1, 6: 1, 8: 1, 10: 2, 11: 2, 13: 4}),
+                           (l.gcb200_matmul_w4, matmul, {1: 1, 4: 1, 5: 1})):
+        for i, off in at.items():
+            assert good[i] == P
+            assert call(*good[:i], P + off, *good[i + 1:]) == INVALID, (call.__name__, i)
+            assert b"misaligned" in l.gcb200_last_error()
+            n += 1
+    assert n == 14
