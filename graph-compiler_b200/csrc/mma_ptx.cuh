@@ -56,13 +56,7 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack_half2(float lo, fl
   return r;
 }
 template <bool BF16> __device__ __forceinline__ uint16_t f32_to_half(float x) { return uint16_t(pack_half2<BF16>(x, 0.f)); }
-// Two e4m3 codes -> two f16 (exact).
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t codes16) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(codes16));
-  return r;
-}
-// Four e4m3 codes -> two pairs of f16, the low halves' first.
+// Four e4m3 codes -> two pairs of f16 (exact), the low halves' first.
 __device__ __forceinline__ void e4m3x4_to_f16x2(uint32_t codes, uint32_t &lo, uint32_t &hi) {
   asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(codes));
 }

@@ -51,7 +51,7 @@ constexpr float kLazy = 8.f;
 struct Cut {
   int seq, unit;
   int first, count;      // blocks with a part of the unit that the border before this block cuts; count 0: it cuts nothing
-  int place;             // of the first block's part: 1 if the unit begins inside its share, 0 with its share
+  int slot;              // of the first block's part (part_slot); the others' are their blocks' first
   int lead;              // the unit's first cut
   int pad[2];
 };
@@ -64,7 +64,7 @@ struct PagedAttParams {
   float *lse, *parts;
   Cut *cuts;
   float scale_log2e;
-  int heads, group, sets, window, blocks, least;   // sets: of query heads per KV head, each the columns of one product
+  int heads, group, sets, window, blocks;   // sets: of query heads per KV head, each the columns of one product
   bool q_aligned, same_strides;
 };
 
@@ -93,12 +93,13 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }   // -inf - -inf would be NaN
 
-// Where tile number `want` of the row of all tiles is: its sequence, the tiles of that sequence's units, and the tile's number from
-// the first tile of the sequence.  All threads of the block call it; pre has room for kThreads + 1.
+// Where a tile of the row of all tiles is.
 struct Place {
   int seq;
-  int64_t rest;     // tiles between the sequence's first and `want`
+  int64_t rest;     // tiles of the sequence before it
 };
+// The number of all tiles; pre (room for kThreads + 1) receives those before each thread's sequences, for one unit.  All threads of
+// the block call it.
 template <int TILE> __device__ __forceinline__ int64_t count_tiles(const PagedAttParams &p, int units, int64_t *pre) {
   const int n = p.c.table.sequences, each = (n + kThreads - 1) / kThreads, s0 = threadIdx.x * each, s1 = min(n, s0 + each);
   int64_t mine = 0;
@@ -123,7 +124,7 @@ template <int TILE> __device__ __forceinline__ int64_t count_tiles(const PagedAt
   if (threadIdx.x == 0) pre[kThreads] = all;
   return all * units;
 }
-// Behind count_tiles; `want` < total.  `found` is shared.
+// The place of tile number `want` < total, behind count_tiles; all threads call it, `found` is shared.
 template <int TILE> __device__ __forceinline__ Place locate(const PagedAttParams &p, int units, const int64_t *pre, int64_t want, Place *found) {
   if (threadIdx.x == 0) *found = Place{};
   __syncthreads();
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
   pdl_wait();
   pdl_launch_dependents();   // behind the wait: what starts now finds everything before this kernel done
 
-  const int64_t total = count_tiles<S::kTile>(p, units, pre), per = share_of(total, p.blocks, p.least);
+  const int64_t total = count_tiles<S::kTile>(p, units, pre), per = share_of(total, p.blocks, 1);
   const int64_t begin = int64_t(blockIdx.x) * per, stop = min(total, begin + per);
   Cut cut{};
 
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
       cut.lead = first_cut(blockIdx.x, per, unit_begin, unit_begin + comp.tiles);
       cut.first = int(unit_begin / per);
       cut.count = int((unit_begin + comp.tiles - 1) / per) - cut.first + 1;
-      cut.place = int(part_slot(cut.first, per, unit_begin) & 1);
+      cut.slot = int(part_slot(cut.first, per, unit_begin));
     }
 
     uint8_t *mine = smem + warp * kStages * S::kSlot;
@@ -634,8 +635,8 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
   if (col >= min(kCols, p.group - set * kCols)) return;
   const int step = together ? kWarps : 1, start = together ? warp : 0, count = (cut.count - start + step - 1) / step;   // this warp's parts
   const int64_t floats = part_floats(kCols, dim);
-  // part i of the unit: the first block's may lie in its second place, every other block's lies in its first
-  const float *rest = p.parts + 2 * int64_t(cut.first) * floats, *first = rest + cut.place * floats;
+  // part i of the unit: every block but the first one continues the unit and has its part in its first slot
+  const float *rest = p.parts + 2 * int64_t(cut.first) * floats, *first = p.parts + cut.slot * floats;
   auto part = [&](int i) {
     const int at = start + i * step;
     return at == 0 ? first : rest + 2 * int64_t(at) * floats;
@@ -765,7 +766,6 @@ template <bool BF16, bool F8, int DP, int NT, bool FULL> void launch(PagedAttPar
     r = std::max(1, n);
   }
   p.blocks = std::min(kMaxBlocks, dev.sm_count * r);
-  p.least = 1;
   launch_dependent(kernel, dim3(unsigned(p.blocks)), S::kBytes, stream, p);
   if (p.blocks > 1) launch_dependent(paged_join_kernel<BF16, F8, NT, (DP + 127) / 128>, dim3(unsigned(p.blocks - 1), 2 * NT), 0, stream, p);
 }
