@@ -16,9 +16,11 @@
 //    nothing that the stream would notice.  P^T goes from the result layout of the first product to the operand layout of the
 //    second by an 8 x 8 transposition in registers.
 //  * The reference m only follows the maximum when that has grown by more than 2^8: one vote per tile instead of a reduction.
-//  * P is rounded once to the type of the product (a second product with the rounding's rest would halve the error, and turn an
-//    infinite value into NaN).  In f16 the reference lies 2^7 below the maximum: without that, tokens below 2^-25 of the largest
-//    would vanish, and a hundred thousand of them may hold a third of a percent of the sum.
+//  * P goes into the product with V as two 16-bit numbers, its upper bits and the rest: to 2^-15 of itself in bf16, 2^-21 in f16, where
+//    one number leaves 2^-8 and 2^-11, and results 1.4 times as far off as their own rounding.  Up to eight query heads to a KV head
+//    this takes 0.7 % at most (2 x 131071 tokens 169.1 -> 170.5 us, 16 x 2048 of 32 heads 89.0 -> 89.4, 8 bits 200.3 -> 198.8), with
+//    sixteen 8 % (219 -> 236).  In f16 the reference lies 2^7 below the maximum: without that, tokens below 2^-25 of the largest would
+//    vanish, and a hundred thousand of them may hold a third of a percent of the sum.
 //  * 8-bit caches become f16 in registers (exact).  Queries are scaled to f16 by a power of two per head.  (Queries as sums of e4m3
 //    numbers against the keys as they are, in e4m3 products, took 236 us where this takes 227.)
 //
@@ -92,6 +94,23 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }   // -inf - -inf would be NaN
+
+// Two numbers of zero and more as the sums of two 16-bit ones each: the upper bits (cut off, returned) and what is left (`rest`).  With
+// INF, where an infinity may meet them, the rest of a number is not zero unless its upper part is: zero times infinity is NaN.
+template <bool BF16, bool INF> __device__ __forceinline__ uint32_t split_half2(float lo, float hi, uint32_t &rest) {
+  constexpr uint32_t kMask = BF16 ? 0xFFFF0000u : 0xFFFFE000u;
+  const float lo_up = __uint_as_float(__float_as_uint(lo) & kMask), hi_up = __uint_as_float(__float_as_uint(hi) & kMask);
+  if constexpr (BF16) {   // 2^-20 of the upper part on top
+    rest = pack_half2<true>(fmaf(lo_up, -(1.f - 0x1p-20f), lo), fmaf(hi_up, -(1.f - 0x1p-20f), hi));
+    return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+  } else {
+    const uint32_t up = pack_half2<false>(lo_up, hi_up);
+    rest = pack_half2<false>(lo - lo_up, hi - hi_up);
+    // at least the smallest number: 2^-31 of the largest weight
+    if constexpr (INF) rest = __vmaxu2(rest, __vminu2(up, 0x00010001u));
+    return up;
+  }
+}
 
 // Where a tile of the row of all tiles is.
 struct Place {
@@ -468,14 +487,18 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
       // ---- P, its sum, and O^T += V^T P^T
 #pragma unroll
       for (int u = 0; u < kSubs; ++u) {
-        uint32_t pt[NT][2];
+        uint32_t pt[NT][2], rt[NT][2];   // the weights' upper bits and the rest
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const float w[4] = {ex2(sc[u][n][0] - ref[n][0]), ex2(sc[u][n][1] - ref[n][1]), ex2(sc[u][n][2] - ref[n][0]), ex2(sc[u][n][3] - ref[n][1])};
           l[n][0] += w[0] + w[2];
           l[n][1] += w[1] + w[3];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) pt[n][h] = movmatrix_trans(pack_half2<kMmaBf16>(w[2 * h], w[2 * h + 1]));
+          for (int h = 0; h < 2; ++h) {
+            uint32_t rest;
+            pt[n][h] = movmatrix_trans(split_half2<kMmaBf16, !F8>(w[2 * h], w[2 * h + 1], rest));
+            rt[n][h] = movmatrix_trans(rest);
+          }
         }
         if constexpr (F8) {
           // chunk j holds head_dim 16 j ..: rows 2 i and 2 i + 1 of the result come from the low and the high byte of its pair i
@@ -492,7 +515,10 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
                 e4m3x4_to_f16x2(t0, a[0], a[1]);
                 e4m3x4_to_f16x2(t1, a[2], a[3]);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma_16816<kMmaBf16>(acc[j + h][n], a, pt[n][0], pt[n][1]);
+                for (int n = 0; n < NT; ++n) {
+                  mma_16816<kMmaBf16>(acc[j + h][n], a, pt[n][0], pt[n][1]);
+                  mma_16816<kMmaBf16>(acc[j + h][n], a, rt[n][0], rt[n][1]);
+                }
               }
             }
           }
@@ -503,7 +529,10 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
               uint32_t a[4];
               ldmatrix_x4_trans(a, vs + pair_at(v_at, u, j));
 #pragma unroll
-              for (int n = 0; n < NT; ++n) mma_16816<kMmaBf16>(acc[j][n], a, pt[n][0], pt[n][1]);
+              for (int n = 0; n < NT; ++n) {
+                mma_16816<kMmaBf16>(acc[j][n], a, pt[n][0], pt[n][1]);
+                mma_16816<kMmaBf16>(acc[j][n], a, rt[n][0], rt[n][1]);
+              }
             }
           }
         }
