@@ -78,19 +78,26 @@ template <bool BF16, int VEC> __device__ __forceinline__ Chunk<VEC> pack(const f
   for (int i = 0; i < (VEC + 1) / 2; ++i) c.w[i] = pack_half2<BF16>(x[2 * i], VEC > 1 ? x[VEC > 1 ? 2 * i + 1 : 0] : 0.f);
   return c;
 }
-// 8-bit codes of x times `by`, the reciprocal of the scale: a quotient within 2^-23 of the border between two codes may go to the
-// other one (a division takes four times the instructions of all the rest).
-template <int VEC, bool ALIGNED> __device__ __forceinline__ void store_e4m3(uint8_t *p, const float (&x)[VEC], float by) {
+// x / scale as a division gives it, from by = 1 / scale: x by is off by a few units in the last place; one step of Newton's method on
+// the remainder, which the fused multiply-add keeps whole, rounds it right (Markstein, IBM J. Res. Dev. 34, 1990).  A division takes
+// four times the instructions of all the rest.  Without the step, quotients on the border between two codes went to either.  Infinities
+// and NaN stay what x by is.
+__device__ __forceinline__ float divided(float x, float scale, float by) {
+  const float y = x * by, z = fmaf(fmaf(-y, scale, x), by, y);
+  return fabsf(y) < 1024.f ? z : y;   // beyond: limited to 448 all the same
+}
+template <int VEC, bool ALIGNED> __device__ __forceinline__ void store_e4m3(uint8_t *p, float (&x)[VEC], float scale, float by) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) x[i] = divided(x[i], scale, by);
   if constexpr (ALIGNED) {
     uint32_t w[VEC / 4];
 #pragma unroll
-    for (int i = 0; i < VEC / 4; ++i)
-      w[i] = f32x2_to_e4m3x2(x[4 * i] * by, x[4 * i + 1] * by) | (f32x2_to_e4m3x2(x[4 * i + 2] * by, x[4 * i + 3] * by) << 16);
+    for (int i = 0; i < VEC / 4; ++i) w[i] = f32x2_to_e4m3x2(x[4 * i], x[4 * i + 1]) | (f32x2_to_e4m3x2(x[4 * i + 2], x[4 * i + 3]) << 16);
     if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t *>(p) = w[0];
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) p[i] = uint8_t(f32x2_to_e4m3x2(x[i] * by, 0.f));
+    for (int i = 0; i < VEC; ++i) p[i] = uint8_t(f32x2_to_e4m3x2(x[i], 0.f));
   }
 }
 
@@ -197,9 +204,9 @@ __global__ void __launch_bounds__(kAppendThreads<VEC>) append_kernel(const __gri
         }
         if (F8 && cached) {
           const float *scales = copied ? c.value_scale : c.key_scale;
-          const float by = scales ? 1.f / scales[head] : 1.f;
-          if (d0 < c.dim) store_e4m3<VEC, ALIGNED>(dst + d0, x, by);
-          if (d1 < c.dim) store_e4m3<VEC, ALIGNED>(dst + d1, y, by);
+          const float scale = scales ? scales[head] : 1.f, by = 1.f / scale;
+          if (d0 < c.dim) store_e4m3<VEC, ALIGNED>(dst + d0, x, scale, by);
+          if (d1 < c.dim) store_e4m3<VEC, ALIGNED>(dst + d1, y, scale, by);
           continue;
         }
         ca = pack<BF16, VEC>(x);

@@ -228,8 +228,8 @@ typedef struct {
  * Token t belongs to sequence sequences[t] (NULL: to sequence t) and stands at positions[t].  With inv_freq (device, f64,
  * rotary_dim / 2 of them; NULL: no rotation) pair i of the first rotary_dim elements of a query or key turns by the angle
  * positions[t] * inv_freq[i], which is formed and reduced in 64 bits; a pair is (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when
- * interleaved.  The rotation is computed in f32 and rounded once; 8-bit caches hold round(x * (1 / scale)), limited
- * to +-448.
+ * interleaved.  The rotation is computed in f32 and rounded once; 8-bit caches hold round(x / scale), the
+ * quotient in f32, limited to +-448.
  * q [tokens][heads][head_dim] (may be NULL) goes to q_out, which may be q itself; strides (elements) are those of tokens and heads;
  * k and v have kv_heads.  A token with a negative sequence or position is padding: its queries are left out too.
  * No two tokens of a call may share a sequence and a position, and no two sequences a page that either appends to. */
