@@ -18,8 +18,9 @@
 //  * The reference m only follows the maximum when that has grown by more than 2^8: one vote per tile instead of a reduction.
 //  * P goes into the product with V as two 16-bit numbers, its upper bits and the rest: to 2^-15 of itself in bf16, 2^-21 in f16, where
 //    one number leaves 2^-8 and 2^-11, and results 1.4 times as far off as their own rounding.  Up to eight query heads to a KV head
-//    this takes 0.7 % at most (2 x 131071 tokens 169.1 -> 170.5 us, 16 x 2048 of 32 heads 89.0 -> 89.4, 8 bits 200.3 -> 198.8), with
-//    sixteen 8 % (219 -> 236).  In f16 the reference lies 2^7 below the maximum: without that, tokens below 2^-25 of the largest would
+//    this takes 0.8 % at most (2 x 131071 tokens 169.1 -> 170.5 us, 16 x 2048 of 32 heads 89.0 -> 89.4), with sixteen 8 % (219 -> 236).
+//    bf16 results over an 8-bit cache do with one f16 number, three bits more than they have themselves: two took 212 us instead of
+//    203 at 128 x 1024..8192 tokens, at the power cap, for the same error.  In f16 the reference lies 2^7 below the maximum: without that, tokens below 2^-25 of the largest would
 //    vanish, and a hundred thousand of them may hold a third of a percent of the sum.
 //  * 8-bit caches become f16 in registers (exact).  Queries are scaled to f16 by a power of two per head.  (Queries as sums of e4m3
 //    numbers against the keys as they are, in e4m3 products, took 236 us where this takes 227.)
@@ -197,6 +198,7 @@ template <bool BF16, bool F8, int DP, int NT, bool FULL>
 __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_attention_kernel(const __grid_constant__ PagedAttParams p) {
   using S = Shape<F8, DP, NT>;
   constexpr bool kMmaBf16 = BF16 && !F8;
+  constexpr bool kSplit = !(F8 && BF16);   // P as two numbers: where one alone has no more bits than the result
   constexpr int kStages = S::kStages, kSteps = DP / 16, kSubs = S::kTokens / 16;
   constexpr float kBelow = kMmaBf16 ? 0.f : 7.f;   // the reference under the maximum: P reaches 2^(kBelow + kLazy), below f16's 2^16
   extern __shared__ __align__(128) uint8_t smem[];
@@ -495,9 +497,13 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
           l[n][1] += w[1] + w[3];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            uint32_t rest;
-            pt[n][h] = movmatrix_trans(split_half2<kMmaBf16, !F8>(w[2 * h], w[2 * h + 1], rest));
-            rt[n][h] = movmatrix_trans(rest);
+            if constexpr (kSplit) {
+              uint32_t rest;
+              pt[n][h] = movmatrix_trans(split_half2<kMmaBf16, !F8>(w[2 * h], w[2 * h + 1], rest));
+              rt[n][h] = movmatrix_trans(rest);
+            } else {
+              pt[n][h] = movmatrix_trans(pack_half2<kMmaBf16>(w[2 * h], w[2 * h + 1]));
+            }
           }
         }
         if constexpr (F8) {
@@ -517,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                   mma_16816<kMmaBf16>(acc[j + h][n], a, pt[n][0], pt[n][1]);
-                  mma_16816<kMmaBf16>(acc[j + h][n], a, rt[n][0], rt[n][1]);
+                  if constexpr (kSplit) mma_16816<kMmaBf16>(acc[j + h][n], a, rt[n][0], rt[n][1]);
                 }
               }
             }
@@ -531,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, Shape<F8, DP, NT>::kResident) paged_
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
                 mma_16816<kMmaBf16>(acc[j][n], a, pt[n][0], pt[n][1]);
-                mma_16816<kMmaBf16>(acc[j][n], a, rt[n][0], rt[n][1]);
+                if constexpr (kSplit) mma_16816<kMmaBf16>(acc[j][n], a, rt[n][0], rt[n][1]);
               }
             }
           }

@@ -5,7 +5,8 @@ Tokens come in pairs of almost the same key and opposite values.  With A the lar
   result    rounded once: u |o| (bf16 2^-8, f16 2^-11)
   scores    dim / 16 products of sixteen, each sum off by 2^-22 of its terms at most, then two roundings: (dim / 16 + 2) 2^-22 A
   weights   2^-22 of the exponential itself; held to 2^-15 + 2^-20 in bf16 (the rest behind eight bits is below 2^-7, eight bits of it
-            are kept) and to 2^-21 in f16, where numbers below its normal range add 2^-23 of a unit that the largest weight is 2^7 of
+            are kept) and to 2^-21 in f16, where numbers below its normal range add 2^-23 of a unit that the largest weight is 2^7 of;
+            bf16 results over an 8-bit cache: one f16 number, half a step of which is 2^-11
   sums      n / 16 products of sixteen: (n / 16 + 2) 2^-22; the softmax's own sum the same
 and the scores' and weights' parts count twice, for the sum that they are divided by."""
 import pytest
@@ -47,7 +48,7 @@ def test_weights_keep_their_bits(dtype, cache, heads, kv, dim, length):
     p = torch.softmax(x, -1)[:, None]
     want, mag, top = (p @ vd)[:, 0], (p @ vd.abs())[:, 0], vd.abs().amax()
     f16 = f8 or dtype == torch.float16
-    weights = (dim / 16 + 2) * 2.0 ** -22 * A + 2.0 ** -22 + (2.0 ** -21 if f16 else 2.0 ** -15 + 2.0 ** -20)
+    weights = (dim / 16 + 2) * 2.0 ** -22 * A + 2.0 ** -22 + (2.0 ** -11 if f8 and dtype == torch.bfloat16 else 2.0 ** -21 if f16 else 2.0 ** -15 + 2.0 ** -20)
     tol = U[dtype] * want.abs() + (2 * weights + 2 * (length / 16 + 2) * 2.0 ** -22) * mag + (length * 2.0 ** -30 * top if f16 else 0) + 2.0 ** -24
     assert ((out - want).abs() <= tol).all(), float(((out - want).abs() / tol).max())
     assert lib.device_error() == 0
