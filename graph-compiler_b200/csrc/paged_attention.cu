@@ -79,12 +79,16 @@ template <bool F8, int DP, int NT> struct Shape {
   static constexpr int kTile = kWarps * kTokens;
   static constexpr int kSlot = 2 * kTokens * kRow;          // a warp's keys and values of one tile
   static constexpr int kCols = 8 * NT;                      // query heads
-  // Three blocks to an SM with 64 KB each, where their registers allow it; else two (one with heads of 256) and three stages.
+  // Blocks to an SM: three where their registers allow it, else two, one with heads of 256.  Three stages where that many blocks then
+  // find room in its 228 KB (each with its statically allocated 3 KB and 1 KB of the driver's), else two.
   static constexpr int kResident = NT == 1 && DP <= 128 ? 3 : DP <= 128 ? 2 : 1;
-  static constexpr int kStages = kResident == 3 && kSlot == 8192 ? 2 : 3;
   static constexpr int kQRow = DP * 2 + 16;                 // bytes, padded against bank conflicts
   static constexpr int kQ = kCols * kQRow;
-  static constexpr int kBytes = kStages * kWarps * kSlot + (kStages + 1) * kQ;
+  static constexpr int bytes(int stages) { return stages * kWarps * kSlot + (stages + 1) * kQ; }
+  static constexpr bool fits(int stages) { return kResident * (bytes(stages) + 4096) <= 228 * 1024; }
+  static constexpr int kStages = fits(3) ? 3 : 2;
+  static constexpr int kBytes = bytes(kStages);
+  static_assert(fits(kStages), "as many blocks to an SM as the registers are shared out for");
   static_assert(kCols * DP * 4 <= kSlot, "a warp's results fit where its tokens were");
 };
 __host__ __device__ __forceinline__ int64_t part_floats(int cols, int dim) { return int64_t(cols) * (dim + 2); }
