@@ -15,9 +15,11 @@
 // tiles; every warp streams blocks of its own through a ring of asynchronous copies that runs on across the tiles.  X lies in shared
 // memory for the whole call.  Where it does not fit, or where there are fewer tiles than SMs, a cluster of 2 to 8 blocks shares
 // the k of its tiles and exchanges f32 sums through distributed shared memory, one tile late, so that nobody waits for them.
-// Measured: 1 x 28672 x 8192 26 us (4.7 TB/s), 8 rows 35, 16 rows 46; 1 x 4096 x 4096 6, of which 4 are launch, first loads and the
-// last sums; 5 x 11001 x 4095 with groups of 32 and zeros 14.  With one row what is left is that fixed time, with sixteen the
-// multiplying warps' instructions: the kernel takes 41 of 47 us with no loads in its loop.
+// Measured: 1 x 28672 x 8192 28 us (4.3 TB/s), 8 rows 36, 16 rows 46, 32 rows 94, 64 rows 185 (a reading of the weights for every 16);
+// 1 x 4096 x 4096 6, of which 4 are launch, first loads and the last sums; 5 x 11001 x 4095 with groups of 32 and zeros 14.  With one
+// row what is left is that fixed time, with sixteen the multiplying warps' instructions: the kernel takes 41 of 47 us with no loads
+// in its loop.  640 threads leave 96 registers: 21 of the 48 variants spill, at most 96 bytes (two tiles, 16 rows, groups of 32: 16 x
+// 28672 x 8192 66 us, groups of 64 61).
 // (1 KB bulk copies instead of the warps' 16-byte ones kept an SM at 12 to 20 bytes a cycle, half of what HBM gives it.)
 #include "decode_ops.h"
 

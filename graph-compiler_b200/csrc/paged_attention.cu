@@ -1,6 +1,7 @@
 // Attention of one new token per sequence over a paged key-value cache:
 //   out = sum_t p_t v_t / sum_t p_t,  p_t = 2^(x_t - m),  x_t = log2(e) scale q . k_t,  m a reference close to max_t x_t
-// with the running reference and sum of an online softmax, so that keys and values are read once.
+// with the running reference and sum of an online softmax, so that keys and values are read once: for up to sixteen query heads to a
+// KV head, eight with head_dim above 128.  More are several sets, each of which reads them again.
 //
 // Bound by HBM: 2 head_dim elements of cache per token and KV head, for 4 head_dim operations per query head, so everything is
 // arranged for an even, unbroken stream of the cache:
@@ -17,19 +18,21 @@
 //    second by an 8 x 8 transposition in registers.
 //  * The reference m only follows the maximum when that has grown by more than 2^8: one vote per tile instead of a reduction.
 //  * P goes into the product with V as two 16-bit numbers, its upper bits and the rest: to 2^-15 of itself in bf16, 2^-21 in f16, where
-//    one number leaves 2^-8 and 2^-11, and results 1.4 times as far off as their own rounding.  Up to eight query heads to a KV head
-//    this takes 0.8 % at most (2 x 131071 tokens 169.1 -> 170.5 us, 16 x 2048 of 32 heads 89.0 -> 89.4), with sixteen 8 % (219 -> 236).
+//    one number leaves 2^-8 and 2^-11, and results 1.4 times as far off as their own rounding.  With one number and with two:
+//    2 x 131071 tokens 168.3 and 169.3 us, 16 x 2048 of 32 heads 87.5 and 87.9, with sixteen query heads to each of them 94.5 and 96.4.
 //    bf16 results over an 8-bit cache do with one f16 number, three bits more than they have themselves: two took 212 us instead of
-//    203 at 128 x 1024..8192 tokens, at the power cap, for the same error.  In f16 the reference lies 2^7 below the maximum: without that, tokens below 2^-25 of the largest would
-//    vanish, and a hundred thousand of them may hold a third of a percent of the sum.
-//  * 8-bit caches become f16 in registers (exact).  Queries are scaled to f16 by a power of two per head.  (Queries as sums of e4m3
-//    numbers against the keys as they are, in e4m3 products, took 236 us where this takes 227.)
+//    203 at 128 x 1024..8192 tokens, at the power cap, for the same error.
+//  * In f16 the reference lies 2^7 below the maximum: without that, tokens below 2^-25 of the largest would vanish, and a hundred
+//    thousand of them may hold a third of a percent of the sum.
+//  * 8-bit caches become f16 in registers (exact).  Queries are scaled to f16 by a power of two per head.
 //
-// Measured, 128-wide heads, eight query heads to a KV head unless said otherwise: 2 x 131071 tokens 166 us (6.4 TB/s; a copy reaches
-// 6.6), 64 x 512..4096 tokens with four heads to a KV head 101 (6.0), 16 x 2048 tokens of 32 heads of their own 87 (6.2), 128 x 1024..8192
-// tokens in 8 bits 195 (6.1, at the power cap: 620 instructions for 8 KB of cache against 340 in 16 bits); sixteen query heads to a
-// KV head, whose registers leave two blocks to an SM, 2 x 131071 214 (5.0).  Few tokens: 1 x 1031 takes 8.8 us, as much on the host (two
-// launches) as on the device; 37 windows of up to 700 tokens 12.4, a chain of latencies (lengths, page numbers, tokens, the warps'
+// Measured through Python with other calls around (two figures where GPUs differ), 128-wide heads, eight query heads to a KV head unless
+// said otherwise: 2 x 131071 tokens 165 to 172 us (6.2 to 6.5 TB/s; a copy reaches 6.6), 64 x 512..4096 tokens with four heads to a KV
+// head 101 to 104 (5.9), 16 x 2048 tokens of 32 heads of their own 88 to 91 (6.0), 128 x 1024..8192 tokens in 8 bits 195 to 203 (5.8 to
+// 6.1, at the power cap: 620 instructions for 8 KB of cache against 360 in 16 bits).  Sixteen query heads to a KV head, whose registers
+// leave two blocks to an SM: 2 x 131071 tokens 166 (6.5), 128 x 1024..8192 in 8 bits 235 (5.0), 64 x 512..4096 111 (5.5); 32 heads, 2 x
+// 131071, 314.  256-wide heads, one sequence of 131071 tokens: 165 (6.5), sixteen to a KV head 315.  Few tokens: 1 x 1031 takes 8.5 us
+// of the device, two launches; 37 windows of up to 700 tokens 12.5, a chain of latencies (lengths, page numbers, tokens, the warps'
 // sums, the join).
 #include "decode_ops.h"
 

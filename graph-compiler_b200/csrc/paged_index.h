@@ -68,8 +68,10 @@ GCB_HD Seen seen_of(const PageTable &t, int length, int window) {
 // of several blocks; each then keeps a part of its softmax, and the parts are joined in the order of the blocks.
 GCB_HD int tiles_of(const Seen &s, int tile) { return (s.end - s.first + tile - 1) / tile; }
 // Large shares are rounded up to fours (never by more than an eighth): where units have 2^n tiles, odd shares leave the blocks at as
-// many different places of a sequence at a time, and 16 sequences x 32 heads x 2048 tokens, 37 tiles to a block, took 104 us instead
-// of 90 with 38 or 40.
+// many different places of a sequence at a time.  Without and with, 32 heads of their own: 16 x 2048 tokens 110 and 90 us, 32 x 1024
+// 112 and 90, 16 x 4096 208 and 176, 8 x 5000 109 and 108.  The blocks that it leaves idle cost less than it gives elsewhere too: 64 x
+// 512..4096 tokens of eight KV heads 102.5 and 103.0, 128 x 1024..8192 in 8 bits 201.8 and 199.2, 2 x 131071 167.9 and 168.6, 8 x 30000
+// 156.0 and 156.4.
 GCB_HD int64_t share_of(int64_t total, int blocks, int least) {
   int64_t per = (total + blocks - 1) / blocks;
   if (per >= 32) per = (per + 3) / 4 * 4;

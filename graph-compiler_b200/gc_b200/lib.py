@@ -421,7 +421,8 @@ def paged_kv_append(q, k, v, key_cache, value_cache, page_table, positions, sequ
     ``page_table`` int32 ``[sequences, pages of a sequence]``, ``positions`` int32 ``[tokens]``, ``sequences`` int32 ``[tokens]``
     (None: token t belongs to sequence t).  A negative sequence or position marks padding, whose rows stay as they are.
     ``inv_freq`` float64 ``[rotary_dim / 2]`` (None: no rotation); ``interleaved``: pairs (2 i, 2 i + 1) instead of halves.
-    ``out`` may be q itself.  Pages outside the cache are not written; :func:`device_error` then gives 9."""
+    ``out`` may be q itself.  Pages outside the cache are not written; :func:`device_error` then gives 9.  No gradient history is kept,
+    here and in the other calls of this file."""
     if q is not None and out is None:
         import torch
 
