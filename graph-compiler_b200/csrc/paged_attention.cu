@@ -17,7 +17,7 @@
 //    nothing that the stream would notice.  P^T goes from the result layout of the first product to the operand layout of the
 //    second by an 8 x 8 transposition in registers.
 //  * The reference m only follows the maximum when that has grown by more than 2^8: one vote per tile instead of a reduction.
-//  * P goes into the product with V as two 16-bit numbers, its upper bits and the rest: to 2^-15 of itself in bf16, 2^-21 in f16, where
+//  * P goes into the product with V as two 16-bit numbers, its upper bits and the rest: to 2^-15 of itself in bf16, 2^-20 in f16, where
 //    one number leaves 2^-8 and 2^-11, and results 1.4 times as far off as their own rounding.  With one number and with two:
 //    2 x 131071 tokens 168.3 and 169.3 us, 16 x 2048 of 32 heads 87.5 and 87.9, with sixteen query heads to each of them 94.5 and 96.4.
 //    bf16 results over an 8-bit cache do with one f16 number, three bits more than they have themselves: two took 212 us instead of
@@ -103,20 +103,21 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }   // -inf - -inf would be NaN
 
-// Two numbers of zero and more as the sums of two 16-bit ones each: the upper bits (cut off, returned) and what is left (`rest`).  With
-// INF, where an infinity may meet them, the rest of a number is not zero unless its upper part is: zero times infinity is NaN.
+// Two numbers of zero and more as the sums of two 16-bit ones each: the upper bits (returned) and what is left (`rest`).  With INF, where
+// an infinity may meet them, both parts are above zero and not just the upper one, since zero times infinity is NaN: the upper bits
+// are those of a little less.  In f16 the steps of a number below 2^-14 (2^-21 of the largest weight) are all 2^-24, and it is rounded to
+// the nearest, whole or in halves: cutting it off, or a rest that is never zero, would add up over many.
 template <bool BF16, bool INF> __device__ __forceinline__ uint32_t split_half2(float lo, float hi, uint32_t &rest) {
-  constexpr uint32_t kMask = BF16 ? 0xFFFF0000u : 0xFFFFE000u;
-  const float lo_up = __uint_as_float(__float_as_uint(lo) & kMask), hi_up = __uint_as_float(__float_as_uint(hi) & kMask);
-  if constexpr (BF16) {   // 2^-20 of the upper part on top
-    rest = pack_half2<true>(fmaf(lo_up, -(1.f - 0x1p-20f), lo), fmaf(hi_up, -(1.f - 0x1p-20f), hi));
+  constexpr float kLess = INF ? 1.f - 0x1p-10f : 1.f, kSmall = INF ? 0.5f : 1.f;
+  if constexpr (BF16) {
+    const float lo_up = __uint_as_float(__float_as_uint(lo) & 0xFFFF0000u), hi_up = __uint_as_float(__float_as_uint(hi) & 0xFFFF0000u);
+    rest = pack_half2<true>(fmaf(lo_up, -(1.f - 0x1p-20f), lo), fmaf(hi_up, -(1.f - 0x1p-20f), hi));   // 2^-20 of the upper part on top
     return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
   } else {
-    const uint32_t up = pack_half2<false>(lo_up, hi_up);
+    const float lo_up = lo < 0x1p-14f ? lo * kSmall : __uint_as_float(__float_as_uint(lo * kLess) & 0xFFFFE000u);
+    const float hi_up = hi < 0x1p-14f ? hi * kSmall : __uint_as_float(__float_as_uint(hi * kLess) & 0xFFFFE000u);
     rest = pack_half2<false>(lo - lo_up, hi - hi_up);
-    // at least the smallest number: 2^-31 of the largest weight
-    if constexpr (INF) rest = __vmaxu2(rest, __vminu2(up, 0x00010001u));
-    return up;
+    return pack_half2<false>(lo_up, hi_up);
   }
 }
 

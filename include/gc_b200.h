@@ -243,7 +243,7 @@ int gcb200_paged_kv_append(const gcb200_paged_cache *cache, const void *q, const
  * lengths (device) count the tokens in the cache, the new one among them.  A sequence of length 0 (or less) gives zeros, and
  * minus infinity in lse.  lse [sequences][heads] f32 (may be NULL) receives log sum_t exp(scale * q . k_t).  Scores, maxima, sums
  * and results are held in f32; exp() of the scores meets the values as the sum of two 16-bit numbers (of it, 2^-15 are lost in bf16
- * and 2^-21 in f16), for bf16 results over an 8-bit cache as one f16 number (2^-11), and the result is rounded once.
+ * and 2^-20 in f16), for bf16 results over an 8-bit cache as one f16 number (2^-11), and the result is rounded once.
  * A length beyond max_pages * page_size is cut to that and recorded as code 9.
  * workspace: device memory, gcb200_paged_attention_workspace() bytes, 16-byte aligned, that no other call in flight uses; nothing
  * in it needs clearing or is kept from one call to the next. */
