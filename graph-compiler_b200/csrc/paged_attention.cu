@@ -28,7 +28,7 @@
 //
 // Measured through Python with other calls around (two figures where GPUs differ), 128-wide heads, eight query heads to a KV head unless
 // said otherwise: 2 x 131071 tokens 165 to 172 us (6.2 to 6.5 TB/s; a copy reaches 6.6), 64 x 512..4096 tokens with four heads to a KV
-// head 101 to 104 (5.9), 16 x 2048 tokens of 32 heads of their own 88 to 91 (6.0), 128 x 1024..8192 tokens in 8 bits 195 to 203 (5.8 to
+// head 101 to 104 (5.9), 16 x 2048 tokens of 32 heads of their own 88 to 91 (6.0), 128 x 1024..8192 tokens in 8 bits 195 to 206 (5.7 to
 // 6.1, at the power cap: 620 instructions for 8 KB of cache against 360 in 16 bits).  Sixteen query heads to a KV head, whose registers
 // leave two blocks to an SM: 2 x 131071 tokens 166 (6.5), 128 x 1024..8192 in 8 bits 235 (5.0), 64 x 512..4096 111 (5.5); 32 heads, 2 x
 // 131071, 314.  256-wide heads, one sequence of 131071 tokens: 165 (6.5), sixteen to a KV head 315.  Few tokens: 1 x 1031 takes 8.5 us
